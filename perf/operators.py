@@ -205,9 +205,9 @@ def _plain_sample(s):
     total = sorted_w.sum(dim=1, keepdim=True)
     keep &= (top_p[:, None] >= 1.0) | (before < top_p[:, None] * total)
     keep &= sorted_w >= min_p[:, None]
-    kept = torch.zeros_like(w).scatter_(1, order, torch.where(keep, sorted_w, 0.0))
-    upto = kept.cumsum(dim=1)
-    drawn = (upto <= s["u"][:, None] * upto[:, -1:]).sum(dim=1)
+    upto = torch.where(keep, sorted_w, 0.0).cumsum(dim=1)
+    place = (upto <= s["u"][:, None] * upto[:, -1:]).sum(dim=1).clamp(max=V - 1)
+    drawn = torch.gather(order, 1, place[:, None])[:, 0]
     return torch.where(temperature > 0.0, drawn, best).int()
 
 
