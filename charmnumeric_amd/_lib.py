@@ -161,6 +161,46 @@ class Tiled(C.Structure):
     ]
 
 
+class RmsNorm(C.Structure):
+    """cnh_rms_norm_args"""
+    _fields_ = [("dtype", C.c_int32), ("rows", C.c_int64), ("cols", C.c_int64), ("x", C.c_void_p),
+                ("x_stride", C.c_int64), ("residual", C.c_void_p), ("residual_stride", C.c_int64),
+                ("residual_out", C.c_void_p), ("residual_out_stride", C.c_int64), ("weight", C.c_void_p),
+                ("eps", C.c_double), ("y", C.c_void_p), ("y_stride", C.c_int64)]
+
+
+class ShortConvolution(C.Structure):
+    """cnh_short_convolution_args"""
+    _fields_ = [("dtype", C.c_int32), ("activation", C.c_int32), ("taps", C.c_int32), ("batch", C.c_int64),
+                ("length", C.c_int64), ("channels", C.c_int64), ("x", C.c_void_p), ("x_batch_stride", C.c_int64),
+                ("x_stride", C.c_int64), ("weight", C.c_void_p), ("bias", C.c_void_p), ("state_in", C.c_void_p),
+                ("state_out", C.c_void_p), ("lengths", C.c_void_p), ("y", C.c_void_p),
+                ("y_batch_stride", C.c_int64), ("y_stride", C.c_int64)]
+
+
+class StateScan(C.Structure):
+    """cnh_state_scan_args"""
+    _fields_ = [("dtype", C.c_int32), ("softplus", C.c_int32), ("batch", C.c_int64), ("length", C.c_int64),
+                ("channels", C.c_int64), ("states", C.c_int64), ("x", C.c_void_p), ("x_batch_stride", C.c_int64),
+                ("x_stride", C.c_int64), ("delta", C.c_void_p), ("delta_batch_stride", C.c_int64),
+                ("delta_stride", C.c_int64), ("z", C.c_void_p), ("z_batch_stride", C.c_int64),
+                ("z_stride", C.c_int64), ("A", C.c_void_p), ("B", C.c_void_p), ("B_batch_stride", C.c_int64),
+                ("B_stride", C.c_int64), ("C", C.c_void_p), ("C_batch_stride", C.c_int64), ("C_stride", C.c_int64),
+                ("skip", C.c_void_p), ("delta_bias", C.c_void_p), ("state_in", C.c_void_p),
+                ("state_out", C.c_void_p), ("lengths", C.c_void_p), ("y", C.c_void_p),
+                ("y_batch_stride", C.c_int64), ("y_stride", C.c_int64), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64)]
+
+
+class SampleTokens(C.Structure):
+    """cnh_sample_tokens_args"""
+    _fields_ = [("dtype", C.c_int32), ("top_k", C.c_int32), ("rows", C.c_int64), ("vocab", C.c_int64),
+                ("logits", C.c_void_p), ("stride", C.c_int64), ("u", C.c_void_p), ("temperature", C.c_double),
+                ("top_p", C.c_double), ("min_p", C.c_double), ("temperatures", C.c_void_p),
+                ("top_ks", C.c_void_p), ("top_ps", C.c_void_p), ("min_ps", C.c_void_p), ("out", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 def _lib_path():
     here = os.path.dirname(os.path.abspath(__file__))
     return os.path.join(here, "libcnhip.so")
@@ -278,6 +318,15 @@ _PROTOS = {
     "cnh_fill_cg_matrix": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int64,
                                      C.c_int64, C.c_int64, C.c_uint64, C.c_void_p]),
 }
+
+_PROTOS.update({
+    "cnh_rms_norm": (C.c_int, [C.POINTER(RmsNorm), C.c_void_p]),
+    "cnh_short_convolution": (C.c_int, [C.POINTER(ShortConvolution), C.c_void_p]),
+    "cnh_state_scan": (C.c_int, [C.POINTER(StateScan), C.c_void_p]),
+    "cnh_state_scan_workspace": (C.c_int64, [C.POINTER(StateScan)]),
+    "cnh_sample_tokens": (C.c_int, [C.POINTER(SampleTokens), C.c_void_p]),
+    "cnh_sample_tokens_workspace": (C.c_int64, [C.POINTER(SampleTokens)]),
+})
 
 # Host executor (include/cnexec.h).
 _i32p = C.POINTER(C.c_int32)

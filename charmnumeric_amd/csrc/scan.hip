@@ -1,0 +1,467 @@
+// Selective state space scan: every channel of every sequence carries `states` numbers from token to
+// token,
+//   s_t = softplus(delta_t + delta_bias)                      (or delta_t + delta_bias as it is)
+//   h_t[n] = exp(s_t A[n]) h_(t-1)[n] + s_t B_t[n] x_t,        n < states
+//   y_t = (sum_n C_t[n] h_t[n] + skip x_t) z_t sigmoid(z_t)
+// with A per channel and B, C shared by the channels of a token. One token per sequence is the same
+// call with length 1.
+//
+// A lane owns NPL states of one channel in registers and walks the tokens; S neighbouring lanes share a
+// channel with more states than that and add their parts of y over the lanes of a row. With S = 1 a
+// wavefront is 64 neighbouring channels, x, delta, z and y move as whole lines, and B_t and C_t are the
+// same for all lanes, so they come through the scalar cache and cost no vector register or LDS read.
+//
+// Per token and channel: 4 elements of memory and, per state, one exponential and five operations.
+// A batch too small to fill the device is cut along the tokens: the recurrence is linear in h, so a
+// piece of the sequence is summed up by the state it leaves when it starts from zero and by the sum of
+// its steps (its decay is exp(A sum s)); a short pass over the pieces gives each its first state, and
+// all pieces then run at once. That costs the exponentials twice, which is why it is left out as soon
+// as the batch fills the device by itself.
+#include "sequence.h"
+
+#include <algorithm>
+
+using namespace cnh;
+
+namespace {
+
+template <typename T>
+struct ScanParams {
+    int64_t batch, length, channels;
+    int states, softplus;
+    const T *x, *delta, *z;
+    int64_t x_bs, x_s, delta_bs, delta_s, z_bs, z_s;
+    const T* A;
+    const T *B, *C;
+    int64_t B_bs, B_s, C_bs, C_s;
+    const T *skip, *delta_bias;
+    const T* state_in;
+    T* state_out;
+    const int32_t* lengths;
+    T* y;
+    int64_t y_bs, y_s;
+    int64_t piece;  // tokens per piece
+    int pieces;     // 1: no cut
+    T* carry;       // [batch][pieces][states][channels]: the state a piece leaves, then the one it starts from
+    T* steps;       // [batch][pieces][channels]: sum of a piece's steps
+};
+
+// exp(s A) with what depends on A alone taken out of the loop: the 32-bit form is one multiplication
+// and the hardware's base-2 exponential (1 ulp); rounding A log2(e) shifts the exponent by at most
+// |s A| 2^-24, which the decay's own size makes harmless.
+__device__ __forceinline__ float rate_of(float a) { return a * 1.44269504088896341f; }
+__device__ __forceinline__ double rate_of(double a) { return a; }
+__device__ __forceinline__ float decay(float s, float rate) { return __builtin_amdgcn_exp2f(s * rate); }
+__device__ __forceinline__ double decay(double s, double rate) { return exp(s * rate); }
+
+// log(1 + e^v). In 32 bits log(u) e / (u - 1) with u = 1 + e^v rounded: the rounding of u cancels.
+__device__ __forceinline__ float softplus(float v) {
+    const float e = __builtin_amdgcn_exp2f(v * 1.44269504088896341f), u = 1.0f + e, d = u - 1.0f;
+    const float l = __builtin_amdgcn_logf(u) * 0.693147180559945309f;
+    const float r = d == 0.0f ? e : l * (e * __builtin_amdgcn_rcpf(d));
+    return v > 20.0f ? v : r;
+}
+__device__ __forceinline__ double softplus(double v) { return v > 40.0 ? v : log1p(exp(v)); }
+
+// v of the lane that a row operation of the vector unit pairs this one with
+template <int CTRL>
+__device__ __forceinline__ float partner(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double partner(double v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, true);
+    return __hiloint2double(hi, lo);
+}
+// Sum over S neighbouring lanes, in every one of them.
+template <int S, typename T>
+__device__ __forceinline__ T lanes_sum(T v) {
+    if (S >= 2)
+        v += partner<0xB1>(v); // quad_perm [1,0,3,2]
+    if (S >= 4)
+        v += partner<0x4E>(v); // quad_perm [2,3,0,1]
+    if (S >= 8)
+        v += partner<0x141>(v); // row_half_mirror
+    if (S >= 16)
+        v += partner<0x140>(v); // row_mirror
+    return v;
+}
+
+// Memory that no kernel in flight writes, for loads at addresses the whole wavefront shares.
+template <typename T>
+using Uniform = const __attribute__((address_space(4))) T;
+
+// NPL states (n0 .. n0 + NPL) of one token's B or C. FULL: all of them exist, the rows of A and of the
+// states are aligned for wide accesses and, with S > 1, those of B and C too.
+template <typename T, int NPL, int S, bool FULL>
+__device__ __forceinline__ void load_states(T (&v)[NPL], const T* row, int n0, int states) {
+    if constexpr (S == 1) {
+        Uniform<T>* u = (Uniform<T>*)(uintptr_t)row;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i)
+            v[i] = FULL ? u[i] : i < states ? u[i] : T(0);
+    } else if constexpr (FULL) {
+        Pack<T, NPL> q;
+        load_pack(q, row + n0);
+#pragma unroll
+        for (int i = 0; i < NPL; ++i)
+            v[i] = q.v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < NPL; ++i)
+            v[i] = n0 + i < states ? row[n0 + i] : T(0);
+    }
+}
+
+// NPL states of a lane's own channel, from a row of `states` elements.
+template <typename T, int NPL, bool FULL>
+__device__ __forceinline__ void own_states(Pack<T, NPL>& v, const T* row, int n0, int states) {
+    if constexpr (FULL) {
+        load_pack(v, row + n0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NPL; ++i)
+            v.v[i] = n0 + i < states ? row[n0 + i] : T(0);
+    }
+}
+
+// PARTIAL: what a piece leaves when it starts from zero; otherwise the scan itself.
+template <typename T, int NPL, int S, bool FULL, bool PARTIAL>
+__global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
+    constexpr int AHEAD = 4; // tokens whose x, delta and z are on their way while others are worked on
+    const int64_t lane = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t d_own = lane / S;
+    const bool live = d_own < p.channels;
+    // lanes past the last channel work on the last one and store nothing: the wavefront stays whole
+    const int64_t d = live ? d_own : p.channels - 1;
+    const int n0 = (int)(lane % S) * NPL;
+    const bool first = n0 == 0;
+    const int64_t piece = blockIdx.y;
+    Pack<T, NPL> rate;
+    own_states<T, NPL, FULL>(rate, p.A + d * p.states, n0, p.states);
+#pragma unroll
+    for (int i = 0; i < NPL; ++i)
+        rate.v[i] = rate_of(rate.v[i]);
+    const T bias = p.delta_bias ? p.delta_bias[d] : T(0), skip = p.skip ? p.skip[d] : T(0);
+
+    for (int64_t b = blockIdx.z; b < p.batch; b += gridDim.z) {
+        const int64_t n = tokens_of(p.lengths, b, p.length);
+        const int64_t begin = piece * p.piece, stop = std::min(begin + p.piece, p.length), end = std::min(stop, n);
+        const T* xp = p.x + b * p.x_bs + d;
+        const T* dp = p.delta + b * p.delta_bs + d;
+        const T* zp = p.z ? p.z + b * p.z_bs + d : nullptr;
+        const T* Bp = p.B + b * p.B_bs;
+        const T* Cp = p.C + b * p.C_bs;
+        T* yp = p.y + b * p.y_bs + d;
+        T* slot = p.carry + ((b * p.pieces + piece) * p.states + n0) * p.channels + d;
+        Pack<T, NPL> h = {};
+        if (!PARTIAL) {
+            if (p.pieces > 1) {
+#pragma unroll
+                for (int i = 0; i < NPL; ++i)
+                    h.v[i] = FULL || n0 + i < p.states ? slot[(int64_t)i * p.channels] : T(0);
+            } else if (p.state_in) {
+                own_states<T, NPL, FULL>(h, p.state_in + (b * p.channels + d) * p.states, n0, p.states);
+            }
+        }
+        T steps = 0;
+        T xs[AHEAD], ds[AHEAD], zs[AHEAD];
+        auto fetch = [&](int64_t t, int u) {
+            const bool in = t < end;
+            xs[u] = in ? xp[t * p.x_s] : T(0);
+            ds[u] = in ? dp[t * p.delta_s] : T(0);
+            zs[u] = !PARTIAL && zp && in ? zp[t * p.z_s] : T(0);
+        };
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            fetch(begin + u, u);
+        for (int64_t t0 = begin; t0 < end; t0 += AHEAD) {
+            T xc[AHEAD], dc[AHEAD], zc[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                xc[u] = xs[u];
+                dc[u] = ds[u];
+                zc[u] = zs[u];
+                fetch(t0 + AHEAD + u, u);
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int64_t t = t0 + u;
+                if (t >= end)
+                    break;
+                T s = dc[u] + bias;
+                if (p.softplus)
+                    s = softplus(s);
+                const T sx = s * xc[u];
+                T Bt[NPL];
+                load_states<T, NPL, S, FULL>(Bt, Bp + t * p.B_s, n0, p.states);
+                if constexpr (PARTIAL) {
+                    steps += s;
+#pragma unroll
+                    for (int i = 0; i < NPL; ++i)
+                        h.v[i] = decay(s, rate.v[i]) * h.v[i] + sx * Bt[i];
+                } else {
+                    T Ct[NPL], sum = 0;
+                    load_states<T, NPL, S, FULL>(Ct, Cp + t * p.C_s, n0, p.states);
+#pragma unroll
+                    for (int i = 0; i < NPL; ++i) {
+                        h.v[i] = decay(s, rate.v[i]) * h.v[i] + sx * Bt[i];
+                        sum += Ct[i] * h.v[i];
+                    }
+                    sum = lanes_sum<S>(sum) + skip * xc[u];
+                    if (zp)
+                        sum *= silu(zc[u]);
+                    if (first && live)
+                        yp[t * p.y_s] = sum;
+                }
+            }
+        }
+        if constexpr (PARTIAL) {
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < NPL; ++i)
+                    if (FULL || n0 + i < p.states)
+                        slot[(int64_t)i * p.channels] = h.v[i];
+                if (first)
+                    p.steps[(b * p.pieces + piece) * p.channels + d] = steps;
+            }
+        } else {
+            if (first && live)
+                for (int64_t t = std::max(begin, end); t < stop; ++t)
+                    yp[t * p.y_s] = T(0);
+            if (p.state_out && piece == p.pieces - 1 && live) {
+                T* row = p.state_out + (b * p.channels + d) * p.states + n0;
+                if constexpr (FULL) {
+                    store_pack(h, row);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NPL; ++i)
+                        if (n0 + i < p.states)
+                            row[i] = h.v[i];
+                }
+            }
+        }
+    }
+}
+
+// One lane per channel and state: the state each piece starts from, in place of the one it leaves.
+// The loads of a group of pieces do not depend on each other and are issued together; without that the
+// pass would wait for memory once per piece.
+template <typename T>
+__global__ __launch_bounds__(256) void carry_kernel(ScanParams<T> p) {
+    constexpr int GROUP = 16;
+    const int64_t d = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (d >= p.channels)
+        return;
+    const int n = blockIdx.y;
+    const T rate = rate_of(p.A[d * p.states + n]);
+    for (int64_t b = blockIdx.z; b < p.batch; b += gridDim.z) {
+        T h = p.state_in ? p.state_in[(b * p.channels + d) * p.states + n] : T(0);
+        for (int c0 = 0; c0 < p.pieces; c0 += GROUP) {
+            T left[GROUP], steps[GROUP];
+#pragma unroll
+            for (int i = 0; i < GROUP; ++i) {
+                const int64_t c = b * p.pieces + c0 + i;
+                const bool in = c0 + i < p.pieces - 1; // nothing starts behind the last piece
+                left[i] = in ? p.carry[(c * p.states + n) * p.channels + d] : T(0);
+                steps[i] = in ? p.steps[c * p.channels + d] : T(0);
+            }
+#pragma unroll
+            for (int i = 0; i < GROUP; ++i) {
+                if (c0 + i >= p.pieces)
+                    break;
+                p.carry[((b * p.pieces + c0 + i) * p.states + n) * p.channels + d] = h;
+                h = decay(steps[i], rate) * h + left[i];
+            }
+        }
+    }
+}
+
+// States per lane, lanes per channel and pieces of a call: host arithmetic on its sizes alone, so that
+// the workspace it needs can be asked for without a device.
+struct Plan {
+    int npl, lanes;
+    int64_t piece;
+    int pieces;
+    int64_t bytes;
+};
+
+Plan plan_of(const cnh_state_scan_args* a) {
+    Plan q;
+    const int64_t N = a->states;
+    if (a->length <= 16 || N <= 4)
+        q.npl = N <= 64 ? 4 : 16;
+    else
+        q.npl = 16;
+    q.lanes = 1;
+    while (q.npl * q.lanes < N)
+        q.lanes *= 2;
+    const int64_t waves = a->batch * ((a->channels * q.lanes + 63) / 64);
+    constexpr int64_t kWanted = 4096; // four wavefronts on each of 256 x 4 vector units
+    q.pieces = 1;
+    if (waves > 0 && waves <= kWanted / 2)
+        q.pieces = (int)std::max<int64_t>(1, std::min(kWanted / waves, a->length / 32));
+    q.piece = std::max<int64_t>(1, (a->length + q.pieces - 1) / q.pieces);
+    if (a->length > 0)
+        q.pieces = (int)((a->length + q.piece - 1) / q.piece);
+    const int64_t esz = dtype_size(a->dtype);
+    q.bytes = q.pieces > 1 ? a->batch * q.pieces * (N + 1) * a->channels * esz : 0;
+    return q;
+}
+
+template <typename T, int NPL, int S, bool FULL>
+int launch(const ScanParams<T>& p, hipStream_t st) {
+    // one wavefront per workgroup spreads a prompt's few long-running wavefronts evenly; a launch of
+    // single tokens has many short ones
+    const int threads = p.length <= 16 ? 256 : 64;
+    const unsigned gx = (unsigned)((p.channels * S + threads - 1) / threads);
+    const unsigned gz = (unsigned)std::min<int64_t>(p.batch, 65535);
+    if (p.pieces > 1) {
+        scan_kernel<T, NPL, S, FULL, true><<<dim3(gx, p.pieces - 1, gz), threads, 0, st>>>(p);
+        carry_kernel<T><<<dim3((unsigned)((p.channels + 255) / 256), p.states, gz), 256, 0, st>>>(p);
+    }
+    scan_kernel<T, NPL, S, FULL, false><<<dim3(gx, p.pieces, gz), threads, 0, st>>>(p);
+    CNH_HIP(hipGetLastError());
+    return 0;
+}
+
+template <typename T, int NPL, int S>
+int launch_full(const ScanParams<T>& p, bool wide, hipStream_t st) {
+    const bool own = aligned_to(p.A, 16) && aligned_to(p.state_in, 16) && aligned_to(p.state_out, 16);
+    if (p.states == NPL * S && own && (S == 1 || wide))
+        return launch<T, NPL, S, true>(p, st);
+    return launch<T, NPL, S, false>(p, st);
+}
+
+template <typename T>
+int run(const cnh_state_scan_args* a, const Plan& q, hipStream_t st) {
+    ScanParams<T> p;
+    auto in = [](const void* v) { return static_cast<const T*>(v); };
+    p.batch = a->batch;
+    p.length = a->length;
+    p.channels = a->channels;
+    p.states = (int)a->states;
+    p.softplus = a->softplus;
+    p.x = in(a->x), p.x_bs = a->x_batch_stride, p.x_s = a->x_stride;
+    p.delta = in(a->delta), p.delta_bs = a->delta_batch_stride, p.delta_s = a->delta_stride;
+    p.z = in(a->z), p.z_bs = a->z_batch_stride, p.z_s = a->z_stride;
+    p.A = in(a->A);
+    p.B = in(a->B), p.B_bs = a->B_batch_stride, p.B_s = a->B_stride;
+    p.C = in(a->C), p.C_bs = a->C_batch_stride, p.C_s = a->C_stride;
+    p.skip = in(a->skip);
+    p.delta_bias = in(a->delta_bias);
+    p.state_in = in(a->state_in);
+    p.state_out = static_cast<T*>(a->state_out);
+    p.lengths = a->lengths;
+    p.y = static_cast<T*>(a->y), p.y_bs = a->y_batch_stride, p.y_s = a->y_stride;
+    p.piece = q.piece;
+    p.pieces = q.pieces;
+    p.carry = static_cast<T*>(a->workspace);
+    p.steps = p.carry ? p.carry + p.batch * p.pieces * p.states * p.channels : nullptr;
+    constexpr int W = Wide<T>::n;
+    auto fits = [&](const void* ptr, int64_t outer, int64_t inner) {
+        return aligned_to(ptr, 16) && (p.batch == 1 || outer % W == 0) && (p.length <= 1 || inner % W == 0);
+    };
+    const bool wide = fits(p.B, p.B_bs, p.B_s) && fits(p.C, p.C_bs, p.C_s);
+    if (q.npl == 4) {
+        switch (q.lanes) {
+        case 1: return launch_full<T, 4, 1>(p, wide, st);
+        case 2: return launch_full<T, 4, 2>(p, wide, st);
+        case 4: return launch_full<T, 4, 4>(p, wide, st);
+        case 8: return launch_full<T, 4, 8>(p, wide, st);
+        default: return launch_full<T, 4, 16>(p, wide, st);
+        }
+    }
+    switch (q.lanes) {
+    case 1: return launch_full<T, 16, 1>(p, wide, st);
+    case 2: return launch_full<T, 16, 2>(p, wide, st);
+    case 4: return launch_full<T, 16, 4>(p, wide, st);
+    case 8: return launch_full<T, 16, 8>(p, wide, st);
+    default: return launch_full<T, 16, 16>(p, wide, st);
+    }
+}
+
+int check_sizes(const cnh_state_scan_args* a, const char* call) {
+    CNH_CHECK(a != nullptr, -2, "%s: null arguments", call);
+    if (int rc = check_float_type(a->dtype, call))
+        return rc;
+    CNH_CHECK(a->batch >= 0 && a->length >= 0 && a->channels >= 0, -2, "%s: batch %lld, length %lld, channels %lld", call,
+              (long long)a->batch, (long long)a->length, (long long)a->channels);
+    CNH_CHECK(a->states >= 1 && a->states <= 256, -3, "%s: %lld states; 1 to 256 are supported", call,
+              (long long)a->states);
+    CNH_CHECK(a->softplus == 0 || a->softplus == 1, -2, "%s: softplus %d is neither 0 nor 1", call, a->softplus);
+    CNH_CHECK(a->batch < ((int64_t)1 << 31) && a->length < ((int64_t)1 << 31) && a->channels < ((int64_t)1 << 24), -3,
+              "%s: batch %lld, length %lld (below 2^31), channels %lld (below 2^24)", call, (long long)a->batch,
+              (long long)a->length, (long long)a->channels);
+    return 0;
+}
+
+} // namespace
+
+extern "C" int64_t cnh_state_scan_workspace(const cnh_state_scan_args* a) {
+    if (int rc = check_sizes(a, "cnh_state_scan_workspace"))
+        return rc;
+    if (a->batch == 0 || a->channels == 0)
+        return 0;
+    return plan_of(a).bytes;
+}
+
+extern "C" int cnh_state_scan(const cnh_state_scan_args* a, cnh_stream s) {
+    const char* call = "cnh_state_scan";
+    if (int rc = check_sizes(a, call))
+        return rc;
+    if (a->batch == 0 || a->channels == 0 || (a->length == 0 && !a->state_out))
+        return 0;
+    CNH_CHECK(a->A && (a->length == 0 || (a->x && a->delta && a->B && a->C && a->y)), -2,
+              "%s: null x, delta, A, B, C or y", call);
+    const int esz = dtype_size(a->dtype);
+    const int64_t D = a->channels, N = a->states;
+    auto rows = [&](const char* what, const void* ptr, int64_t bs, int64_t st, int64_t cols) {
+        return Extent{what, ptr, span_of(a->batch, bs, a->length, st, cols) * esz};
+    };
+    const __int128 state = (__int128)a->batch * D * N * esz;
+    CNH_CHECK(state < ((__int128)1 << 62), -3, "%s: the states do not fit any memory", call);
+    const Plan q = plan_of(a);
+    const Extent y = rows("y", a->y, a->y_batch_stride, a->y_stride, D),
+                 out{"state_out", a->state_out, (int64_t)state}, in{"state_in", a->state_in, (int64_t)state},
+                 ws{"workspace", a->workspace, q.bytes}, len{"lengths", a->lengths, a->batch * 4};
+    const Extent reads[] = {rows("x", a->x, a->x_batch_stride, a->x_stride, D),
+                            rows("delta", a->delta, a->delta_batch_stride, a->delta_stride, D),
+                            rows("z", a->z, a->z_batch_stride, a->z_stride, D),
+                            rows("B", a->B, a->B_batch_stride, a->B_stride, N),
+                            rows("C", a->C, a->C_batch_stride, a->C_stride, N),
+                            {"A", a->A, D * N * esz},
+                            {"skip", a->skip, D * esz},
+                            {"delta_bias", a->delta_bias, D * esz}};
+    for (const Extent* e : {&y, &out, &in})
+        if (int rc = check_extent(*e, esz, call))
+            return rc;
+    for (const Extent& e : reads)
+        if (int rc = check_extent(e, esz, call))
+            return rc;
+    if (int rc = check_extent(len, 4, call))
+        return rc;
+    CNH_CHECK(q.bytes == 0 || (a->workspace && a->workspace_bytes >= q.bytes), -2,
+              "%s: a workspace of %lld bytes is needed, %lld given", call, (long long)q.bytes,
+              (long long)(a->workspace ? a->workspace_bytes : 0));
+    CNH_CHECK(q.bytes == 0 || aligned_to(a->workspace, 16), -2, "%s: the workspace is not aligned to 16 bytes", call);
+    CNH_CHECK(a->length == 0 || rows_apart(a->batch, a->y_batch_stride, a->length, a->y_stride, D), -2,
+              "%s: rows of y overlap", call);
+    const Extent* writes[] = {&y, &out, &ws};
+    for (const Extent* w : writes) {
+        for (const Extent& e : reads)
+            CNH_CHECK(!overlap(*w, e), -2, "%s: %s overlaps %s", call, w->what, e.what);
+        CNH_CHECK(!overlap(*w, len), -2, "%s: %s overlaps lengths", call, w->what);
+        CNH_CHECK(w == &out || !overlap(*w, in), -2, "%s: %s overlaps state_in", call, w->what);
+        CNH_CHECK(w == &out || !overlap(*w, out), -2, "%s: %s overlaps state_out", call, w->what);
+    }
+    CNH_CHECK(!overlap(y, ws), -2, "%s: y overlaps the workspace", call);
+    CNH_CHECK(!overlap(out, in) || out.ptr == in.ptr, -2, "%s: state_out overlaps state_in without being the same", call);
+    if (int rc = ensure_init())
+        return rc;
+    DeviceScope dev;
+    if (int rc = dev.enter())
+        return rc;
+    return a->dtype == CNH_F32 ? run<float>(a, q, as_stream(s)) : run<double>(a, q, as_stream(s));
+}

@@ -482,6 +482,123 @@ int cnh_fill_uniform_tile(double* out, int ndims, const int64_t* ext, const int6
                           const int64_t* global_shape, uint64_t seed, uint64_t stream_id, double lo,
                           double hi, cnh_stream s);
 
+/* ---- operators of recurrent sequence models (no upstream counterpart: upstream's model is the LSTM
+ *      forward written in array statements, examples/lstm_forward.py:40-49, and its only reduction is the
+ *      1-D dot, src/executor_reduce.cpp:9-12) ----
+ * fp32 and fp64. Rows are contiguous, strides count elements, optional operands may be null. A call
+ * queues its work on `s` and returns; it allocates nothing and keeps nothing, so it may be captured into a
+ * graph once cnh_init has run. Sizes of zero are no work. Outputs must not overlap inputs or each
+ * other (-2) except where it says so, each operand taken from its first element to its last;
+ * `lengths` (device, one per sequence) holds how many of its `length` tokens a sequence has, values
+ * outside [0, length] being held to it: rows of y behind them are zeros, whatever x holds there, and
+ * the state is that behind the last token that counts. */
+
+/* r = x + residual; y = r / sqrt(mean over the row of r^2 + eps) * weight. residual, residual_out and
+ * weight (ones) are optional; residual_out receives r and may be the residual itself. */
+typedef struct cnh_rms_norm_args {
+    int32_t dtype;
+    int64_t rows, cols;
+    const void* x;
+    int64_t x_stride;
+    const void* residual;
+    int64_t residual_stride;
+    void* residual_out;
+    int64_t residual_out_stride;
+    const void* weight;
+    double eps;
+    void* y;
+    int64_t y_stride;
+} cnh_rms_norm_args;
+int cnh_rms_norm(const cnh_rms_norm_args* a, cnh_stream s);
+
+/* Causal convolution of every channel along its tokens with 1 to 8 taps:
+ *   y[b, t, c] = act(bias[c] + sum over k < taps of weight[k, c] * x[b, t - (taps - 1) + k, c])
+ * act: activation 0 none, 1 v * sigmoid(v). The rows in front of the first token come from
+ * state_in (batch, taps - 1, channels; null: zeros); state_out receives the last taps - 1 rows of each
+ * sequence, state included, and may be state_in itself. length 1 is one token per sequence. */
+typedef struct cnh_short_convolution_args {
+    int32_t dtype, activation, taps;
+    int64_t batch, length, channels;
+    const void* x;
+    int64_t x_batch_stride, x_stride;
+    const void* weight;
+    const void* bias;
+    const void* state_in;
+    void* state_out;
+    const int32_t* lengths;
+    void* y;
+    int64_t y_batch_stride, y_stride;
+} cnh_short_convolution_args;
+int cnh_short_convolution(const cnh_short_convolution_args* a, cnh_stream s);
+
+/* Selective state space scan, 1 to 256 states per channel:
+ *   step = delta + delta_bias, through log(1 + exp(.)) with softplus = 1
+ *   h[b, c, n] = exp(step[b, t, c] * A[c, n]) * h[b, c, n] + step[b, t, c] * B[b, t, n] * x[b, t, c]
+ *   y[b, t, c] = (sum over n of C[b, t, n] * h[b, c, n] + skip[c] * x[b, t, c]) * z * sigmoid(z),
+ *                z = z[b, t, c]
+ * delta_bias, skip and z are optional (0, 0, no factor). h starts from state_in (batch, channels,
+ * states; null: zeros) and is left in state_out, which may be state_in itself. length 1 is one token
+ * per sequence. A batch that does not fill the device by itself is cut along the tokens: `workspace`
+ * (device, 16-byte aligned, undefined contents before and after) then holds the bytes
+ * cnh_state_scan_workspace asks for (it looks at the type and the sizes alone and needs no device).
+ * Calls that may run at the same time need workspaces of their own, captured graphs among them. The
+ * cut depends on the sizes alone; an output's last bits can differ between batch sizes. */
+typedef struct cnh_state_scan_args {
+    int32_t dtype, softplus;
+    int64_t batch, length, channels, states;
+    const void* x;
+    int64_t x_batch_stride, x_stride;
+    const void* delta;
+    int64_t delta_batch_stride, delta_stride;
+    const void* z;
+    int64_t z_batch_stride, z_stride;
+    const void* A;
+    const void* B;
+    int64_t B_batch_stride, B_stride;
+    const void* C;
+    int64_t C_batch_stride, C_stride;
+    const void* skip;
+    const void* delta_bias;
+    const void* state_in;
+    void* state_out;
+    const int32_t* lengths;
+    void* y;
+    int64_t y_batch_stride, y_stride;
+    void* workspace;
+    int64_t workspace_bytes;
+} cnh_state_scan_args;
+int64_t cnh_state_scan_workspace(const cnh_state_scan_args* a);
+int cnh_state_scan(const cnh_state_scan_args* a, cnh_stream s);
+
+/* One word per row of logits (1 to 2^22 words), drawn with the random number u[row] of [0, 1):
+ *   w = exp((logit - largest logit of the row) / temperature)
+ * top_k > 0 keeps the k largest (ties: the lowest indices); then top_p < 1 keeps the shortest run of
+ * those, in descending order, whose sum reaches top_p of theirs (one word at least); then min_p > 0 keeps
+ * w >= min_p. out[row] is the first word, in descending order, at which the running sum of the kept
+ * weights exceeds u[row] times their sum. A temperature of 0 takes the largest logit (ties: the lowest
+ * index). -inf and NaN are never drawn; a row of nothing else gives -1. Weights are compared as
+ * multiples of 2^-45 (of 2^-40 for 2^22 words), words more than 32 temperatures below the largest logit have none.
+ * The scalars apply to every row; an array (device, one entry per row) takes the place of its scalar,
+ * and an entry outside its range is held to it (a temperature that is not positive takes the largest
+ * logit). `workspace` as for cnh_state_scan. */
+typedef struct cnh_sample_tokens_args {
+    int32_t dtype, top_k;
+    int64_t rows, vocab;
+    const void* logits;
+    int64_t stride;
+    const double* u;
+    double temperature, top_p, min_p;
+    const double* temperatures;
+    const int32_t* top_ks;
+    const double* top_ps;
+    const double* min_ps;
+    int32_t* out;
+    void* workspace;
+    int64_t workspace_bytes;
+} cnh_sample_tokens_args;
+int64_t cnh_sample_tokens_workspace(const cnh_sample_tokens_args* a);
+int cnh_sample_tokens(const cnh_sample_tokens_args* a, cnh_stream s);
+
 #ifdef __cplusplus
 }
 #endif
