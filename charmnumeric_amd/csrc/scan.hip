@@ -20,6 +20,7 @@
 #include "sequence.h"
 
 #include <algorithm>
+#include <type_traits>
 
 using namespace cnh;
 
@@ -28,6 +29,7 @@ namespace {
 template <typename T>
 struct ScanParams {
     int64_t batch, length, channels;
+    int64_t first_batch; // of this launch
     int states, softplus;
     const T *x, *delta, *z;
     int64_t x_bs, x_s, delta_bs, delta_s, z_bs, z_s;
@@ -40,7 +42,7 @@ struct ScanParams {
     const int32_t* lengths;
     T* y;
     int64_t y_bs, y_s;
-    int64_t piece;  // tokens per piece
+    int64_t piece;  // tokens per piece (a single token: sequences per workgroup)
     int pieces;     // 1: no cut
     T* carry;       // [batch][pieces][states][channels]: the state a piece leaves, then the one it starts from
     T* steps;       // [batch][pieces][channels]: sum of a piece's steps
@@ -88,6 +90,17 @@ __device__ __forceinline__ T lanes_sum(T v) {
     return v;
 }
 
+// Element of a row that the wavefront shares, by the lane's byte offset (below 2^28): the row's address
+// stays in scalar registers.
+template <typename T>
+__device__ __forceinline__ const T& at(const T* row, uint32_t bytes) {
+    return *reinterpret_cast<const T*>(reinterpret_cast<const char*>(row) + bytes);
+}
+template <typename T>
+__device__ __forceinline__ T& at(T* row, uint32_t bytes) {
+    return *reinterpret_cast<T*>(reinterpret_cast<char*>(row) + bytes);
+}
+
 // Memory that no kernel in flight writes, for loads at addresses the whole wavefront shares.
 template <typename T>
 using Uniform = const __attribute__((address_space(4))) T;
@@ -126,154 +139,281 @@ __device__ __forceinline__ void own_states(Pack<T, NPL>& v, const T* row, int n0
     }
 }
 
+template <typename T, int NPL, bool FULL>
+__device__ __forceinline__ void store_states(const Pack<T, NPL>& v, T* row, int n0, int states) {
+    if constexpr (FULL) {
+        store_pack(v, row + n0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NPL; ++i)
+            if (n0 + i < states)
+                row[n0 + i] = v.v[i];
+    }
+}
+
 // PARTIAL: what a piece leaves when it starts from zero; otherwise the scan itself.
 template <typename T, int NPL, int S, bool FULL, bool PARTIAL>
-__global__ __launch_bounds__(256) void scan_kernel(ScanParams<T> p) {
+__global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
     constexpr int AHEAD = 4; // tokens whose x, delta and z are on their way while others are worked on
-    const int64_t lane = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t d_own = lane / S;
-    const bool live = d_own < p.channels;
+    const uint32_t lane = blockIdx.x * 64 + threadIdx.x; // below 2^28: 16 lanes for each of 2^24 channels
+    const uint32_t d_own = lane / S;
+    const bool live = d_own < (uint32_t)p.channels;
     // lanes past the last channel work on the last one and store nothing: the wavefront stays whole
-    const int64_t d = live ? d_own : p.channels - 1;
+    const uint32_t d = live ? d_own : (uint32_t)p.channels - 1;
     const int n0 = (int)(lane % S) * NPL;
+    const uint32_t off = d * (uint32_t)sizeof(T);
     const bool first = n0 == 0;
     const int64_t piece = blockIdx.y;
     Pack<T, NPL> rate;
-    own_states<T, NPL, FULL>(rate, p.A + d * p.states, n0, p.states);
+    own_states<T, NPL, FULL>(rate, p.A + (int64_t)d * p.states, n0, p.states);
 #pragma unroll
     for (int i = 0; i < NPL; ++i)
         rate.v[i] = rate_of(rate.v[i]);
     const T bias = p.delta_bias ? p.delta_bias[d] : T(0), skip = p.skip ? p.skip[d] : T(0);
 
-    for (int64_t b = blockIdx.z; b < p.batch; b += gridDim.z) {
-        const int64_t n = tokens_of(p.lengths, b, p.length);
-        const int64_t begin = piece * p.piece, stop = std::min(begin + p.piece, p.length), end = std::min(stop, n);
-        const T* xp = p.x + b * p.x_bs + d;
-        const T* dp = p.delta + b * p.delta_bs + d;
-        const T* zp = p.z ? p.z + b * p.z_bs + d : nullptr;
-        const T* Bp = p.B + b * p.B_bs;
-        const T* Cp = p.C + b * p.C_bs;
-        T* yp = p.y + b * p.y_bs + d;
-        T* slot = p.carry + ((b * p.pieces + piece) * p.states + n0) * p.channels + d;
-        Pack<T, NPL> h = {};
-        if (!PARTIAL) {
-            if (p.pieces > 1) {
+    const int64_t b = p.first_batch + blockIdx.z;
+    const int64_t n = tokens_of(p.lengths, b, p.length);
+    const int64_t begin = piece * p.piece, stop = std::min(begin + p.piece, p.length), end = std::min(stop, n);
+    // rows: the same for the whole wavefront; a lane adds its channel
+    const T* xp = p.x + b * p.x_bs;
+    const T* dp = p.delta + b * p.delta_bs;
+    const T* zp = p.z ? p.z + b * p.z_bs : nullptr;
+    // without a gate the loads of z repeat those of x: cheaper than a branch around each
+    const T* zq = zp ? zp : xp;
+    const int64_t zq_s = zp ? p.z_s : p.x_s;
+    T* yp = p.y + b * p.y_bs;
+    T* slot = p.carry + ((b * p.pieces + piece) * p.states + n0) * p.channels + d;
+    Pack<T, NPL> h = {};
+    if (!PARTIAL) {
+        if (p.pieces > 1) {
+#pragma unroll
+            for (int i = 0; i < NPL; ++i)
+                h.v[i] = FULL || n0 + i < p.states ? slot[(int64_t)i * p.channels] : T(0);
+        } else if (p.state_in) {
+            own_states<T, NPL, FULL>(h, p.state_in + (b * p.channels + d) * p.states, n0, p.states);
+        }
+    }
+    T steps = 0;
+    // M tokens from t0 on; their steps and gates first, so that the branches on what the call has come once
+    const T *Bt_row = p.B + b * p.B_bs + begin * p.B_s, *Ct_row = p.C + b * p.C_bs + begin * p.C_s;
+    T* y_row = yp + begin * p.y_s;
+    auto tokens = [&](auto count, const T* xc, const T* dc, const T* zc) {
+        constexpr int M = decltype(count)::value;
+        T s[M], gate[M];
+#pragma unroll
+        for (int u = 0; u < M; ++u)
+            s[u] = dc[u] + bias;
+        if (p.softplus)
+#pragma unroll
+            for (int u = 0; u < M; ++u)
+                s[u] = softplus(s[u]);
+        if (!PARTIAL && zp) {
+#pragma unroll
+            for (int u = 0; u < M; ++u)
+                gate[u] = silu(zc[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < M; ++u) {
+            const T sx = s[u] * xc[u];
+            T Bt[NPL];
+            load_states<T, NPL, S, FULL>(Bt, Bt_row, n0, p.states);
+            Bt_row += p.B_s;
+            if constexpr (PARTIAL) {
+                steps += s[u];
 #pragma unroll
                 for (int i = 0; i < NPL; ++i)
-                    h.v[i] = FULL || n0 + i < p.states ? slot[(int64_t)i * p.channels] : T(0);
-            } else if (p.state_in) {
-                own_states<T, NPL, FULL>(h, p.state_in + (b * p.channels + d) * p.states, n0, p.states);
+                    h.v[i] = decay(s[u], rate.v[i]) * h.v[i] + sx * Bt[i];
+            } else {
+                T Ct[NPL], sum = 0;
+                load_states<T, NPL, S, FULL>(Ct, Ct_row, n0, p.states);
+                Ct_row += p.C_s;
+#pragma unroll
+                for (int i = 0; i < NPL; ++i) {
+                    h.v[i] = decay(s[u], rate.v[i]) * h.v[i] + sx * Bt[i];
+                    sum += Ct[i] * h.v[i];
+                }
+                sum = lanes_sum<S>(sum) + skip * xc[u];
+                if (zp)
+                    sum *= gate[u];
+                if (first && live)
+                    at(y_row, off) = sum;
+                y_row += p.y_s;
             }
         }
-        T steps = 0;
+    };
+    // Whole groups of tokens, the next group's x, delta and z on their way meanwhile, then what is left.
+    // Behind the last group the last one is fetched again: no branch stands between a load and its wait.
+    const T *x_row = xp + begin * p.x_s, *d_row = dp + begin * p.delta_s, *z_row = zq + begin * zq_s;
+    const int groups = end > begin ? (int)((end - begin) / AHEAD) : 0, rest = end > begin ? (int)((end - begin) % AHEAD) : 0;
+    if (groups > 0) {
         T xs[AHEAD], ds[AHEAD], zs[AHEAD];
-        auto fetch = [&](int64_t t, int u) {
-            const bool in = t < end;
-            xs[u] = in ? xp[t * p.x_s] : T(0);
-            ds[u] = in ? dp[t * p.delta_s] : T(0);
-            zs[u] = !PARTIAL && zp && in ? zp[t * p.z_s] : T(0);
-        };
+        auto fetch = [&]() {
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-            fetch(begin + u, u);
-        for (int64_t t0 = begin; t0 < end; t0 += AHEAD) {
+            for (int u = 0; u < AHEAD; ++u) {
+                xs[u] = at(x_row + u * p.x_s, off);
+                ds[u] = at(d_row + u * p.delta_s, off);
+                zs[u] = PARTIAL ? T(0) : at(z_row + u * zq_s, off);
+            }
+        };
+        fetch();
+        for (int g = 1; g <= groups; ++g) {
             T xc[AHEAD], dc[AHEAD], zc[AHEAD];
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 xc[u] = xs[u];
                 dc[u] = ds[u];
                 zc[u] = zs[u];
-                fetch(t0 + AHEAD + u, u);
             }
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const int64_t t = t0 + u;
-                if (t >= end)
-                    break;
-                T s = dc[u] + bias;
-                if (p.softplus)
-                    s = softplus(s);
-                const T sx = s * xc[u];
-                T Bt[NPL];
-                load_states<T, NPL, S, FULL>(Bt, Bp + t * p.B_s, n0, p.states);
-                if constexpr (PARTIAL) {
-                    steps += s;
-#pragma unroll
-                    for (int i = 0; i < NPL; ++i)
-                        h.v[i] = decay(s, rate.v[i]) * h.v[i] + sx * Bt[i];
-                } else {
-                    T Ct[NPL], sum = 0;
-                    load_states<T, NPL, S, FULL>(Ct, Cp + t * p.C_s, n0, p.states);
-#pragma unroll
-                    for (int i = 0; i < NPL; ++i) {
-                        h.v[i] = decay(s, rate.v[i]) * h.v[i] + sx * Bt[i];
-                        sum += Ct[i] * h.v[i];
-                    }
-                    sum = lanes_sum<S>(sum) + skip * xc[u];
-                    if (zp)
-                        sum *= silu(zc[u]);
-                    if (first && live)
-                        yp[t * p.y_s] = sum;
-                }
-            }
+            const int on = g < groups ? AHEAD : 0;
+            x_row += on * p.x_s;
+            d_row += on * p.delta_s;
+            z_row += on * zq_s;
+            fetch();
+            tokens(std::integral_constant<int, AHEAD>(), xc, dc, zc);
         }
-        if constexpr (PARTIAL) {
-            if (live) {
+        x_row += AHEAD * p.x_s;
+        d_row += AHEAD * p.delta_s;
+        z_row += AHEAD * zq_s;
+    }
+    for (int r = 0; r < rest; ++r) {
+        const T xc = at(x_row, off), dc = at(d_row, off), zc = PARTIAL ? T(0) : at(z_row, off);
+        x_row += p.x_s;
+        d_row += p.delta_s;
+        z_row += zq_s;
+        tokens(std::integral_constant<int, 1>(), &xc, &dc, &zc);
+    }
+    if constexpr (PARTIAL) {
+        if (live) {
 #pragma unroll
-                for (int i = 0; i < NPL; ++i)
-                    if (FULL || n0 + i < p.states)
-                        slot[(int64_t)i * p.channels] = h.v[i];
-                if (first)
-                    p.steps[(b * p.pieces + piece) * p.channels + d] = steps;
-            }
-        } else {
-            if (first && live)
-                for (int64_t t = std::max(begin, end); t < stop; ++t)
-                    yp[t * p.y_s] = T(0);
-            if (p.state_out && piece == p.pieces - 1 && live) {
-                T* row = p.state_out + (b * p.channels + d) * p.states + n0;
-                if constexpr (FULL) {
-                    store_pack(h, row);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NPL; ++i)
-                        if (n0 + i < p.states)
-                            row[i] = h.v[i];
-                }
-            }
+            for (int i = 0; i < NPL; ++i)
+                if (FULL || n0 + i < p.states)
+                    slot[(int64_t)i * p.channels] = h.v[i];
+            if (first)
+                p.steps[(b * p.pieces + piece) * p.channels + d] = steps;
+        }
+    } else {
+        if (first && live)
+            for (int64_t t = std::max(begin, end); t < stop; ++t)
+                (yp + t * p.y_s)[d] = T(0);
+        if (p.state_out && piece == p.pieces - 1 && live) {
+            store_states<T, NPL, FULL>(h, p.state_out + (b * p.channels + d) * p.states, n0, p.states);
         }
     }
 }
 
-// One lane per channel and state: the state each piece starts from, in place of the one it leaves.
-// The loads of a group of pieces do not depend on each other and are issued together; without that the
-// pass would wait for memory once per piece.
+// The state each piece starts from, in place of the one it leaves: 64 channels of one state per
+// workgroup, SEGMENTS x GROUP pieces a round. A lane loads its GROUP pieces at once, folds them to one,
+// takes what the segments before it leave from shared memory and walks its pieces again in registers;
+// one lane per channel that walks all pieces by itself waits for memory once per GROUP of them instead
+// (128 pieces of 2048 x 16 fp32 states: 22.5 us).
+constexpr int kSegments = 8;
 template <typename T>
-__global__ __launch_bounds__(256) void carry_kernel(ScanParams<T> p) {
-    constexpr int GROUP = 16;
-    const int64_t d = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (d >= p.channels)
-        return;
+__global__ __launch_bounds__(64 * kSegments) void carry_kernel(ScanParams<T> p) {
+    constexpr int GROUP = 8;
+    __shared__ T left_by[kSegments][64], steps_of[kSegments][64];
+    const int seg = threadIdx.y, lane = threadIdx.x;
+    const int64_t own = (int64_t)blockIdx.x * 64 + lane;
+    const bool live = own < p.channels;
+    const int64_t d = live ? own : p.channels - 1;
     const int n = blockIdx.y;
+    const int64_t b = p.first_batch + blockIdx.z;
     const T rate = rate_of(p.A[d * p.states + n]);
-    for (int64_t b = blockIdx.z; b < p.batch; b += gridDim.z) {
-        T h = p.state_in ? p.state_in[(b * p.channels + d) * p.states + n] : T(0);
-        for (int c0 = 0; c0 < p.pieces; c0 += GROUP) {
-            T left[GROUP], steps[GROUP];
+    T start = p.state_in ? p.state_in[(b * p.channels + d) * p.states + n] : T(0); // of the round
+    for (int c0 = 0; c0 < p.pieces; c0 += kSegments * GROUP) {
+        const int c1 = c0 + seg * GROUP;
+        T left[GROUP], steps[GROUP];
 #pragma unroll
-            for (int i = 0; i < GROUP; ++i) {
-                const int64_t c = b * p.pieces + c0 + i;
-                const bool in = c0 + i < p.pieces - 1; // nothing starts behind the last piece
-                left[i] = in ? p.carry[(c * p.states + n) * p.channels + d] : T(0);
-                steps[i] = in ? p.steps[c * p.channels + d] : T(0);
-            }
+        for (int i = 0; i < GROUP; ++i) {
+            const int64_t c = b * p.pieces + c1 + i;
+            const bool in = c1 + i < p.pieces - 1; // nothing starts behind the last piece
+            left[i] = in ? p.carry[(c * p.states + n) * p.channels + d] : T(0);
+            steps[i] = in ? p.steps[c * p.channels + d] : T(0);
+        }
+        T h = 0, sum = 0;
 #pragma unroll
-            for (int i = 0; i < GROUP; ++i) {
-                if (c0 + i >= p.pieces)
-                    break;
-                p.carry[((b * p.pieces + c0 + i) * p.states + n) * p.channels + d] = h;
-                h = decay(steps[i], rate) * h + left[i];
+        for (int i = 0; i < GROUP; ++i) {
+            h = decay(steps[i], rate) * h + left[i];
+            sum += steps[i];
+        }
+        left_by[seg][lane] = h;
+        steps_of[seg][lane] = sum;
+        __syncthreads();
+        T at = start;
+        h = start;
+        for (int s = 0; s < kSegments; ++s) {
+            if (s == seg)
+                h = at;
+            at = decay(steps_of[s][lane], rate) * at + left_by[s][lane];
+        }
+        start = at;
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) {
+            if (c1 + i < p.pieces && live)
+                p.carry[((b * p.pieces + c1 + i) * p.states + n) * p.channels + d] = h;
+            h = decay(steps[i], rate) * h + left[i];
+        }
+        __syncthreads(); // the next round writes the shared memory again
+    }
+}
+
+// One token per sequence. The states are what moves: they are read and written once as 16-byte
+// accesses, a lane keeps its channel's A through the sequences of its slice, and the next sequence's
+// operands are on their way while the present one is worked on.
+template <typename T, int NPL, int S, bool FULL>
+__global__ __launch_bounds__(256) void token_kernel(ScanParams<T> p) {
+    const uint32_t lane = blockIdx.x * 256 + threadIdx.x;
+    const uint32_t d_own = lane / S;
+    const bool live = d_own < (uint32_t)p.channels;
+    const uint32_t d = live ? d_own : (uint32_t)p.channels - 1;
+    const int n0 = (int)(lane % S) * NPL;
+    const int64_t begin = blockIdx.y * p.piece, end = std::min(begin + p.piece, p.batch);
+    Pack<T, NPL> rate;
+    own_states<T, NPL, FULL>(rate, p.A + (int64_t)d * p.states, n0, p.states);
+#pragma unroll
+    for (int i = 0; i < NPL; ++i)
+        rate.v[i] = rate_of(rate.v[i]);
+    const T bias = p.delta_bias ? p.delta_bias[d] : T(0), skip = p.skip ? p.skip[d] : T(0);
+    struct Operands {
+        T x, delta, z, B[NPL], C[NPL];
+        Pack<T, NPL> h;
+        bool there;
+    };
+    auto fetch = [&](int64_t b, Operands& o) {
+        o.there = tokens_of(p.lengths, b, 1) > 0;
+        o.x = (p.x + b * p.x_bs)[d];
+        o.delta = (p.delta + b * p.delta_bs)[d];
+        o.z = p.z ? (p.z + b * p.z_bs)[d] : T(0);
+        load_states<T, NPL, S, FULL>(o.B, p.B + b * p.B_bs, n0, p.states);
+        load_states<T, NPL, S, FULL>(o.C, p.C + b * p.C_bs, n0, p.states);
+        o.h = Pack<T, NPL>{};
+        if (p.state_in)
+            own_states<T, NPL, FULL>(o.h, p.state_in + (b * p.channels + d) * p.states, n0, p.states);
+    };
+    Operands next;
+    fetch(begin, next);
+    for (int64_t b = begin; b < end; ++b) {
+        Operands o = next;
+        fetch(std::min(b + 1, end - 1), next);
+        T out = 0;
+        if (o.there) {
+            T s = o.delta + bias;
+            if (p.softplus)
+                s = softplus(s);
+            const T sx = s * o.x;
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) {
+                o.h.v[i] = decay(s, rate.v[i]) * o.h.v[i] + sx * o.B[i];
+                out += o.C[i] * o.h.v[i];
             }
+            out = lanes_sum<S>(out) + skip * o.x;
+            if (p.z)
+                out *= silu(o.z);
+        }
+        if (live) {
+            if (n0 == 0)
+                (p.y + b * p.y_bs)[d] = out;
+            if (p.state_out)
+                store_states<T, NPL, FULL>(o.h, p.state_out + (b * p.channels + d) * p.states, n0, p.states);
         }
     }
 }
@@ -287,41 +427,61 @@ struct Plan {
     int64_t bytes;
 };
 
+constexpr int64_t kUnits = 256 * 4; // vector units of the device
+
 Plan plan_of(const cnh_state_scan_args* a) {
     Plan q;
-    const int64_t N = a->states;
-    if (a->length <= 16 || N <= 4)
-        q.npl = N <= 64 ? 4 : 16;
-    else
-        q.npl = 16;
-    q.lanes = 1;
-    while (q.npl * q.lanes < N)
-        q.lanes *= 2;
-    const int64_t waves = a->batch * ((a->channels * q.lanes + 63) / 64);
-    constexpr int64_t kWanted = 4096; // four wavefronts on each of 256 x 4 vector units
+    const int64_t N = a->states, D = a->channels, L = a->length;
+    auto lanes = [&](int npl) {
+        int s = 1;
+        while (npl * s < N)
+            s *= 2;
+        return s;
+    };
+    auto waves = [&](int s) { return a->batch * ((D * s + 63) / 64); };
+    // Few states per lane spread a small call over more lanes and make a single token's states one
+    // 16-byte access each; many states per lane share a token's step and gate. Few as long as the
+    // pieces of 32 tokens that the call could be cut into would not fill the device with many.
+    const int many = N <= 8 ? 8 : 16;
+    q.npl = many;
+    if (N <= 64 && (N <= 4 || L <= 1 || waves(lanes(many)) * std::max<int64_t>(1, L / 32) < 2 * kUnits))
+        q.npl = 4;
+    q.lanes = lanes(q.npl);
     q.pieces = 1;
-    if (waves > 0 && waves <= kWanted / 2)
-        q.pieces = (int)std::max<int64_t>(1, std::min(kWanted / waves, a->length / 32));
-    q.piece = std::max<int64_t>(1, (a->length + q.pieces - 1) / q.pieces);
-    if (a->length > 0)
-        q.pieces = (int)((a->length + q.piece - 1) / q.piece);
-    const int64_t esz = dtype_size(a->dtype);
-    q.bytes = q.pieces > 1 ? a->batch * q.pieces * (N + 1) * a->channels * esz : 0;
+    const int64_t w = waves(q.lanes);
+    if (L <= 1) {
+        // sequences per slice: eight wavefronts on each vector unit, or what there is
+        const int64_t row = (D * q.lanes + 63) / 64, slices = std::max<int64_t>(1, std::min(a->batch, 8 * kUnits / std::max<int64_t>(row, 1)));
+        q.piece = std::max<int64_t>(1, (a->batch + slices - 1) / slices);
+        q.piece = std::max(q.piece, (a->batch + 65534) / 65535);
+    } else {
+        if (w <= 2 * kUnits && w > 0)
+            q.pieces = (int)std::max<int64_t>(1, std::min(4 * kUnits / w, L / 16));
+        q.piece = (L + q.pieces - 1) / q.pieces;
+        q.pieces = (int)((L + q.piece - 1) / q.piece);
+    }
+    q.bytes = q.pieces > 1 ? a->batch * q.pieces * (N + 1) * D * dtype_size(a->dtype) : 0;
     return q;
 }
 
 template <typename T, int NPL, int S, bool FULL>
-int launch(const ScanParams<T>& p, hipStream_t st) {
-    // one wavefront per workgroup spreads a prompt's few long-running wavefronts evenly; a launch of
-    // single tokens has many short ones
-    const int threads = p.length <= 16 ? 256 : 64;
-    const unsigned gx = (unsigned)((p.channels * S + threads - 1) / threads);
-    const unsigned gz = (unsigned)std::min<int64_t>(p.batch, 65535);
-    if (p.pieces > 1) {
-        scan_kernel<T, NPL, S, FULL, true><<<dim3(gx, p.pieces - 1, gz), threads, 0, st>>>(p);
-        carry_kernel<T><<<dim3((unsigned)((p.channels + 255) / 256), p.states, gz), 256, 0, st>>>(p);
+int launch(ScanParams<T> p, hipStream_t st) {
+    if (p.length == 1) {
+        const dim3 grid((unsigned)((p.channels * S + 255) / 256), (unsigned)((p.batch + p.piece - 1) / p.piece));
+        token_kernel<T, NPL, S, FULL><<<grid, 256, 0, st>>>(p);
+        CNH_HIP(hipGetLastError());
+        return 0;
     }
-    scan_kernel<T, NPL, S, FULL, false><<<dim3(gx, p.pieces, gz), threads, 0, st>>>(p);
+    // one wavefront per workgroup: few long-running wavefronts spread evenly over the device
+    const unsigned gx = (unsigned)((p.channels * S + 63) / 64);
+    for (p.first_batch = 0; p.first_batch < p.batch; p.first_batch += 65535) { // what a grid takes
+        const unsigned gz = (unsigned)std::min<int64_t>(p.batch - p.first_batch, 65535);
+        if (p.pieces > 1) {
+            scan_kernel<T, NPL, S, FULL, true><<<dim3(gx, p.pieces - 1, gz), 64, 0, st>>>(p);
+            carry_kernel<T><<<dim3((unsigned)((p.channels + 63) / 64), p.states, gz), dim3(64, kSegments), 0, st>>>(p);
+        }
+        scan_kernel<T, NPL, S, FULL, false><<<dim3(gx, p.pieces, gz), 64, 0, st>>>(p);
+    }
     CNH_HIP(hipGetLastError());
     return 0;
 }
@@ -373,6 +533,8 @@ int run(const cnh_state_scan_args* a, const Plan& q, hipStream_t st) {
         default: return launch_full<T, 4, 16>(p, wide, st);
         }
     }
+    if (q.npl == 8)
+        return launch_full<T, 8, 1>(p, wide, st);
     switch (q.lanes) {
     case 1: return launch_full<T, 16, 1>(p, wide, st);
     case 2: return launch_full<T, 16, 2>(p, wide, st);
