@@ -10,6 +10,7 @@ from .interface import CharmNumericInterface, LocalCluster
 from .lazy import execute, reset, set_auto_flush
 from .operations import (add, diag, divide, dot, exp, matmul, maxabs_diff, multiply, norm2, subtract, sum,
                          sumsq_diff, tanh, tile)
+from .sequence import rms_norm, short_convolution, state_scan
 
 ndarray = Array
 float32, float64, int32, int64 = _np.float32, _np.float64, _np.int32, _np.int64
@@ -22,6 +23,6 @@ __all__ = [
     "asarray", "copy", "copyto", "create_array", "diag", "divide", "dot", "dtype", "e", "empty",
     "empty_like", "exp", "eye", "execute", "float32", "float64", "full", "full_like", "identity", "int32",
     "int64", "matmul", "maxabs_diff", "multiply", "ndarray", "newaxis", "norm2", "ones", "ones_like", "pi",
-    "random", "reset", "set_auto_flush", "subtract", "sum", "sumsq_diff", "tanh", "tile", "zeros",
-    "zeros_like",
+    "random", "reset", "rms_norm", "set_auto_flush", "short_convolution", "state_scan", "subtract", "sum",
+    "sumsq_diff", "tanh", "tile", "zeros", "zeros_like",
 ]

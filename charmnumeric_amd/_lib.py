@@ -201,6 +201,36 @@ class SampleTokens(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
+class Operand(C.Structure):
+    """cnx_operand"""
+    _fields_ = [("name", C.c_int32), ("region", Region)]
+
+
+class XRmsNorm(C.Structure):
+    """cnx_rms_norm_args"""
+    _fields_ = [("x", Operand), ("residual", C.c_int32), ("weight", C.c_int32), ("y", C.c_int32), ("eps", C.c_double)]
+
+
+class XShortConvolution(C.Structure):
+    """cnx_short_convolution_args"""
+    _fields_ = [("x", Operand), ("weight", C.c_int32), ("bias", C.c_int32), ("state", C.c_int32),
+                ("lengths", C.c_int32), ("y", C.c_int32), ("activation", C.c_int32)]
+
+
+class XStateScan(C.Structure):
+    """cnx_state_scan_args"""
+    _fields_ = [("x", Operand), ("delta", Operand), ("z", Operand), ("B", Operand), ("C", Operand), ("A", C.c_int32),
+                ("skip", C.c_int32), ("delta_bias", C.c_int32), ("state", C.c_int32), ("lengths", C.c_int32),
+                ("y", C.c_int32), ("softplus", C.c_int32)]
+
+
+class XSampleTokens(C.Structure):
+    """cnx_sample_tokens_args"""
+    _fields_ = [("logits", Operand), ("u", C.c_int32), ("temperatures", C.c_int32), ("top_ks", C.c_int32),
+                ("top_ps", C.c_int32), ("min_ps", C.c_int32), ("out", C.c_int32), ("top_k", C.c_int32),
+                ("temperature", C.c_double), ("top_p", C.c_double), ("min_p", C.c_double)]
+
+
 def _lib_path():
     here = os.path.dirname(os.path.abspath(__file__))
     return os.path.join(here, "libcnhip.so")
@@ -344,6 +374,10 @@ _PROTOS.update({
     "cnx_put": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_void_p]),
     "cnx_fill_uniform": (C.c_int, [C.c_void_p, C.c_int, C.c_uint64, C.c_uint64, C.c_double, C.c_double]),
     "cnx_fill_cg_matrix": (C.c_int, [C.c_void_p, C.c_int, C.c_uint64]),
+    "cnx_rms_norm": (C.c_int, [C.c_void_p, C.POINTER(XRmsNorm)]),
+    "cnx_short_convolution": (C.c_int, [C.c_void_p, C.POINTER(XShortConvolution)]),
+    "cnx_state_scan": (C.c_int, [C.c_void_p, C.POINTER(XStateScan)]),
+    "cnx_sample_tokens": (C.c_int, [C.c_void_p, C.POINTER(XSampleTokens)]),
     "cnx_sync": (C.c_int, [C.c_void_p]),
     "cnx_array_info": (C.c_int, [C.c_void_p, C.c_int, C.POINTER(C.c_int), C.POINTER(C.c_int),
                                  C.POINTER(C.c_int), _i32p, _i32p]),

@@ -308,7 +308,8 @@ bool flat_rule(const Ex* ex, int nd, const int32_t* shape, int tile, const int32
     return false;
 }
 
-int make_array(Ex* ex, int name, int ndims, int dtype, const int32_t* shape, bool zero, XArray** out) {
+int make_array(Ex* ex, int name, int ndims, int dtype, const int32_t* shape, bool zero, XArray** out,
+               bool block = false) {
     CNH_CHECK(ndims >= 1 && ndims <= 3, -20, "array %d: unsupported rank %d", name, ndims);
     CNH_CHECK(dtype_size(dtype) != 0, -20, "array %d: unknown dtype %d", name, dtype);
     CNH_CHECK(ex->arrays.find(name) == ex->arrays.end(), -21, "array %d already exists", name);
@@ -345,7 +346,7 @@ int make_array(Ex* ex, int name, int ndims, int dtype, const int32_t* shape, boo
     }
     const int esz = dtype_size(dtype);
     int64_t off = 0;
-    a.flat = flat_rule(ex, ndims, a.shape, a.tile, a.offset);
+    a.flat = (block && ndims > 1) || flat_rule(ex, ndims, a.shape, a.tile, a.offset);
     if (a.flat && ndims == 2) {
         a.pitch[1] = 1;
         a.pitch[0] = a.shape[1];
@@ -402,6 +403,7 @@ int make_array(Ex* ex, int name, int ndims, int dtype, const int32_t* shape, boo
 }
 
 int make_block(Ex* ex, XArray& a);
+int store_as_block(Ex* ex, XArray& a);
 
 int ensure_alt(Ex* ex, XArray& a) {
     if (a.alt)
@@ -3328,6 +3330,11 @@ int make_block(Ex* ex, XArray& a) {
     if (a.flat)
         return 0;
     CNH_CHECK(!a.phased(), -26, "array %d: tiles that do not start at element 0", a.name);
+    return store_as_block(ex, a);
+}
+
+// The same wherever the array's tile grid starts.
+int store_as_block(Ex* ex, XArray& a) {
     const int esz = dtype_size(a.dtype), nd = a.ndims;
     const size_t bytes = (size_t)std::max<int64_t>(((int64_t)a.elems * esz + 255) & ~(int64_t)255, 256);
     void* block = nullptr;
@@ -4672,6 +4679,327 @@ int cnx_fill_cg_matrix(cnx_executor* ex, int name, uint64_t seed) {
             return rc;
     }
     return 0;
+}
+
+// ---- operators of recurrent sequence models --------------------------------------------------------
+// Each is one call of cnhip.h on arrays stored as one row-major block (an operand that is still cut into
+// tiles is laid out as one first, and stays so). They run in program order like a fill or an upload.
+
+namespace {
+
+// An operand as the C entry points take it: address, elements between rows of the last dimension.
+struct SeqOperand {
+    char* ptr = nullptr;
+    int nd = 0, dtype = 0;
+    int64_t ext[3] = {1, 1, 1}, stride[3] = {0, 0, 0};
+};
+
+int seq_operand(Ex* ex, const char* call, const char* what, const cnx_operand& o, SeqOperand* out) {
+    if (o.name == 0)
+        return 0;
+    XArray* a;
+    if (int rc = find_array(ex, o.name, &a, call))
+        return rc;
+    out->nd = a->ndims;
+    out->dtype = a->dtype;
+    int64_t start[3] = {0, 0, 0};
+    for (int d = 0; d < a->ndims; ++d) {
+        out->ext[d] = a->shape[d];
+        if (!o.region.is_global) {
+            const cnh_region& r = o.region;
+            CNH_CHECK(r.ndims == a->ndims && r.step[d] == 1 && r.start[d] >= 0 && r.start[d] < r.stop[d] &&
+                          r.stop[d] <= a->shape[d],
+                      -50, "%s: the region of %s does not fit array %d or has steps", call, what, o.name);
+            start[d] = r.start[d];
+            out->ext[d] = r.stop[d] - r.start[d];
+        }
+    }
+    if (a->ndims > 1 && !a->flat && a->ntiles > 1)
+        if (int rc = store_as_block(ex, *a))
+            return rc;
+    int64_t run = 1, off = 0;
+    for (int d = a->ndims - 1; d >= 0; --d) {
+        out->stride[d] = run;
+        off += start[d] * run;
+        run *= a->shape[d];
+    }
+    out->ptr = static_cast<char*>(a->slab) + off * dtype_size(a->dtype);
+    return 0;
+}
+
+// A whole array of given rank, extents and type (name 0: none).
+int seq_whole(Ex* ex, const char* call, const char* what, int name, int dtype, int nd, const int64_t* ext, void** out) {
+    *out = nullptr;
+    if (name == 0)
+        return 0;
+    cnx_operand o;
+    std::memset(&o, 0, sizeof o);
+    o.name = name;
+    o.region.is_global = 1;
+    SeqOperand v;
+    if (int rc = seq_operand(ex, call, what, o, &v))
+        return rc;
+    bool fits = v.nd == nd && v.dtype == dtype;
+    for (int d = 0; d < nd && fits; ++d)
+        fits = v.ext[d] == ext[d];
+    CNH_CHECK(fits, -50, "%s: %s (array %d) has the wrong rank, extents or element type", call, what, name);
+    *out = v.ptr;
+    return 0;
+}
+
+// batch x length x columns: rank 3, or rank 2 as one token per sequence.
+struct SeqRows {
+    int64_t batch = 0, length = 0, cols = 0, batch_stride = 0, stride = 0;
+    void* ptr = nullptr;
+};
+int seq_rows(Ex* ex, const char* call, const char* what, const cnx_operand& o, int dtype, SeqRows* r) {
+    if (o.name == 0)
+        return 0;
+    SeqOperand v;
+    if (int rc = seq_operand(ex, call, what, o, &v))
+        return rc;
+    CNH_CHECK(v.nd >= 2 && v.dtype == dtype, -50, "%s: %s (array %d) needs rank 2 or 3 and the call's element type", call,
+              what, o.name);
+    r->batch = v.ext[0];
+    r->length = v.nd == 3 ? v.ext[1] : 1;
+    r->cols = v.ext[v.nd - 1];
+    r->batch_stride = v.stride[0];
+    r->stride = v.nd == 3 ? v.stride[1] : v.ext[1];
+    r->ptr = v.ptr;
+    return 0;
+}
+bool same_rows(const SeqRows& a, const SeqRows& b) { return a.batch == b.batch && a.length == b.length; }
+
+int seq_dtype(Ex* ex, const char* call, const cnx_operand& o, int* dtype, int* nd) {
+    XArray* a;
+    if (int rc = find_array(ex, o.name, &a, call))
+        return rc;
+    CNH_CHECK(a->dtype == CNH_F32 || a->dtype == CNH_F64, -50, "%s: array %d is not of a floating-point type", call, o.name);
+    *dtype = a->dtype;
+    *nd = a->ndims;
+    return 0;
+}
+
+// The result array, and its deletion again when the call is refused.
+int seq_result(Ex* ex, int name, int nd, int dtype, const int64_t* ext, XArray** out) {
+    int32_t shape[3] = {1, 1, 1};
+    for (int d = 0; d < nd; ++d)
+        shape[d] = (int32_t)ext[d];
+    return make_array(ex, name, nd, dtype, shape, false, out, true);
+}
+int seq_end(Ex* ex, int rc, int result) {
+    if (rc) {
+        const std::string text = cnh_last_error();
+        drop_array(ex, result);
+        return set_error(rc, "%s", text.c_str());
+    }
+    return 0;
+}
+
+} // namespace
+
+int cnx_rms_norm(cnx_executor* ex, const cnx_rms_norm_args* q) {
+    const char* call = "rms_norm";
+    CNH_CHECK(ex != nullptr && q != nullptr, -2, "null argument");
+    if (int rc = settle(ex))
+        return rc;
+    int dtype, nd;
+    if (int rc = seq_dtype(ex, call, q->x, &dtype, &nd))
+        return rc;
+    SeqOperand x;
+    if (int rc = seq_operand(ex, call, "x", q->x, &x))
+        return rc;
+    cnh_rms_norm_args a;
+    std::memset(&a, 0, sizeof a);
+    a.dtype = dtype;
+    a.rows = nd == 1 ? 1 : nd == 2 ? x.ext[0] : x.ext[0] * x.ext[1];
+    a.cols = x.ext[nd - 1];
+    CNH_CHECK(nd < 3 || x.ext[0] == 1 || x.stride[0] == x.ext[1] * x.stride[1], -50,
+              "%s: the rows of x (array %d) are not evenly spaced", call, q->x.name);
+    a.x = x.ptr;
+    a.x_stride = nd == 1 ? x.ext[0] : x.stride[nd - 2];
+    a.eps = q->eps;
+    void *res, *weight;
+    if (int rc = seq_whole(ex, call, "residual", q->residual, dtype, nd, x.ext, &res))
+        return rc;
+    if (int rc = seq_whole(ex, call, "weight", q->weight, dtype, 1, &a.cols, &weight))
+        return rc;
+    a.residual = a.residual_out = res;
+    a.residual_stride = a.residual_out_stride = a.y_stride = a.cols;
+    a.weight = weight;
+    XArray* y;
+    if (int rc = seq_result(ex, q->y, nd, dtype, x.ext, &y))
+        return rc;
+    a.y = y->slab;
+    if (ex->trace_on) ex->log("rms_norm " + std::to_string(q->x.name) + " -> " + std::to_string(q->y) + " rows=" + std::to_string(a.rows));
+    return ex->dry ? 0 : seq_end(ex, cnh_rms_norm(&a, ex->stream), q->y);
+}
+
+int cnx_short_convolution(cnx_executor* ex, const cnx_short_convolution_args* q) {
+    const char* call = "short_convolution";
+    CNH_CHECK(ex != nullptr && q != nullptr, -2, "null argument");
+    if (int rc = settle(ex))
+        return rc;
+    int dtype, nd;
+    if (int rc = seq_dtype(ex, call, q->x, &dtype, &nd))
+        return rc;
+    SeqRows x;
+    if (int rc = seq_rows(ex, call, "x", q->x, dtype, &x))
+        return rc;
+    XArray* w;
+    if (int rc = find_array(ex, q->weight, &w, call))
+        return rc;
+    CNH_CHECK(w->ndims == 2 && w->shape[0] <= 8, -50, "%s: weight (array %d) needs rank 2 and at most 8 rows", call, q->weight);
+    cnh_short_convolution_args a;
+    std::memset(&a, 0, sizeof a);
+    a.dtype = dtype;
+    a.activation = q->activation;
+    a.taps = w->shape[0];
+    a.batch = x.batch, a.length = x.length, a.channels = x.cols;
+    a.x = x.ptr, a.x_batch_stride = x.batch_stride, a.x_stride = x.stride;
+    const int64_t wext[2] = {a.taps, a.channels}, sext[3] = {a.batch, a.taps - 1, a.channels};
+    void *weight, *bias, *state, *lengths;
+    if (int rc = seq_whole(ex, call, "weight", q->weight, dtype, 2, wext, &weight))
+        return rc;
+    if (int rc = seq_whole(ex, call, "bias", q->bias, dtype, 1, wext + 1, &bias))
+        return rc;
+    if (int rc = seq_whole(ex, call, "state", q->state, dtype, 3, sext, &state))
+        return rc;
+    if (int rc = seq_whole(ex, call, "lengths", q->lengths, CNH_I32, 1, &a.batch, &lengths))
+        return rc;
+    a.weight = weight, a.bias = bias, a.state_in = a.state_out = state;
+    a.lengths = static_cast<const int32_t*>(lengths);
+    const int64_t ext3[3] = {a.batch, a.length, a.channels}, ext2[2] = {a.batch, a.channels};
+    XArray* y;
+    if (int rc = seq_result(ex, q->y, nd, dtype, nd == 3 ? ext3 : ext2, &y))
+        return rc;
+    a.y = y->slab, a.y_batch_stride = a.length * a.channels, a.y_stride = a.channels;
+    if (ex->trace_on) ex->log("short_convolution " + std::to_string(q->x.name) + " -> " + std::to_string(q->y) + " taps=" + std::to_string(a.taps));
+    return ex->dry ? 0 : seq_end(ex, cnh_short_convolution(&a, ex->stream), q->y);
+}
+
+int cnx_state_scan(cnx_executor* ex, const cnx_state_scan_args* q) {
+    const char* call = "state_scan";
+    CNH_CHECK(ex != nullptr && q != nullptr, -2, "null argument");
+    if (int rc = settle(ex))
+        return rc;
+    int dtype, nd;
+    if (int rc = seq_dtype(ex, call, q->x, &dtype, &nd))
+        return rc;
+    SeqRows x, delta, z, B, C;
+    const cnx_operand* ops[5] = {&q->x, &q->delta, &q->z, &q->B, &q->C};
+    const char* names[5] = {"x", "delta", "z", "B", "C"};
+    SeqRows* rows[5] = {&x, &delta, &z, &B, &C};
+    for (int i = 0; i < 5; ++i) {
+        CNH_CHECK(ops[i]->name != 0 || i == 2, -2, "%s: no %s", call, names[i]);
+        if (int rc = seq_rows(ex, call, names[i], *ops[i], dtype, rows[i]))
+            return rc;
+        CNH_CHECK(!rows[i]->ptr || (same_rows(*rows[i], x) && rows[i]->cols == (i < 3 ? x.cols : B.cols)), -50,
+                  "%s: %s (array %d) does not fit x or B", call, names[i], ops[i]->name);
+    }
+    cnh_state_scan_args a;
+    std::memset(&a, 0, sizeof a);
+    a.dtype = dtype;
+    a.softplus = q->softplus;
+    a.batch = x.batch, a.length = x.length, a.channels = x.cols, a.states = B.cols;
+    a.x = x.ptr, a.x_batch_stride = x.batch_stride, a.x_stride = x.stride;
+    a.delta = delta.ptr, a.delta_batch_stride = delta.batch_stride, a.delta_stride = delta.stride;
+    a.z = z.ptr, a.z_batch_stride = z.batch_stride, a.z_stride = z.stride;
+    a.B = B.ptr, a.B_batch_stride = B.batch_stride, a.B_stride = B.stride;
+    a.C = C.ptr, a.C_batch_stride = C.batch_stride, a.C_stride = C.stride;
+    const int64_t aext[2] = {a.channels, a.states}, sext[3] = {a.batch, a.channels, a.states};
+    void *A, *skip, *bias, *state, *lengths;
+    CNH_CHECK(q->A != 0, -2, "%s: no A", call);
+    if (int rc = seq_whole(ex, call, "A", q->A, dtype, 2, aext, &A))
+        return rc;
+    if (int rc = seq_whole(ex, call, "skip", q->skip, dtype, 1, aext, &skip))
+        return rc;
+    if (int rc = seq_whole(ex, call, "delta_bias", q->delta_bias, dtype, 1, aext, &bias))
+        return rc;
+    if (int rc = seq_whole(ex, call, "state", q->state, dtype, 3, sext, &state))
+        return rc;
+    if (int rc = seq_whole(ex, call, "lengths", q->lengths, CNH_I32, 1, &a.batch, &lengths))
+        return rc;
+    a.A = A, a.skip = skip, a.delta_bias = bias, a.state_in = a.state_out = state;
+    a.lengths = static_cast<const int32_t*>(lengths);
+    const int64_t need = cnh_state_scan_workspace(&a);
+    if (need < 0)
+        return (int)need;
+    const int64_t ext3[3] = {a.batch, a.length, a.channels}, ext2[2] = {a.batch, a.channels};
+    XArray* y;
+    if (int rc = seq_result(ex, q->y, nd, dtype, nd == 3 ? ext3 : ext2, &y))
+        return rc;
+    a.y = y->slab, a.y_batch_stride = a.length * a.channels, a.y_stride = a.channels;
+    if (ex->trace_on) ex->log("state_scan " + std::to_string(q->x.name) + " -> " + std::to_string(q->y) + " states=" + std::to_string(a.states));
+    // the workspace goes back to the free list at once: what takes it next runs behind this on the stream
+    const size_t bytes = ((size_t)need + 255) & ~(size_t)255;
+    if (bytes) {
+        if (int rc = slab_alloc(ex, bytes, false, &a.workspace))
+            return seq_end(ex, rc, q->y);
+        a.workspace_bytes = need;
+    }
+    const int rc = ex->dry ? 0 : cnh_state_scan(&a, ex->stream);
+    if (bytes)
+        slab_release(ex, bytes, a.workspace);
+    return seq_end(ex, rc, q->y);
+}
+
+int cnx_sample_tokens(cnx_executor* ex, const cnx_sample_tokens_args* q) {
+    const char* call = "sample_tokens";
+    CNH_CHECK(ex != nullptr && q != nullptr, -2, "null argument");
+    if (int rc = settle(ex))
+        return rc;
+    int dtype, nd;
+    if (int rc = seq_dtype(ex, call, q->logits, &dtype, &nd))
+        return rc;
+    SeqOperand l;
+    if (int rc = seq_operand(ex, call, "logits", q->logits, &l))
+        return rc;
+    CNH_CHECK(nd <= 2, -50, "%s: logits (array %d) have rank %d", call, q->logits.name, nd);
+    cnh_sample_tokens_args a;
+    std::memset(&a, 0, sizeof a);
+    a.dtype = dtype;
+    a.rows = nd == 2 ? l.ext[0] : 1;
+    a.vocab = l.ext[nd - 1];
+    a.logits = l.ptr;
+    a.stride = nd == 2 ? l.stride[0] : l.ext[0];
+    a.top_k = q->top_k;
+    a.temperature = q->temperature, a.top_p = q->top_p, a.min_p = q->min_p;
+    CNH_CHECK(q->u != 0, -2, "%s: no random numbers", call);
+    void *u, *t, *k, *p, *m;
+    if (int rc = seq_whole(ex, call, "u", q->u, CNH_F64, 1, &a.rows, &u))
+        return rc;
+    if (int rc = seq_whole(ex, call, "temperature", q->temperatures, CNH_F64, 1, &a.rows, &t))
+        return rc;
+    if (int rc = seq_whole(ex, call, "top_k", q->top_ks, CNH_I32, 1, &a.rows, &k))
+        return rc;
+    if (int rc = seq_whole(ex, call, "top_p", q->top_ps, CNH_F64, 1, &a.rows, &p))
+        return rc;
+    if (int rc = seq_whole(ex, call, "min_p", q->min_ps, CNH_F64, 1, &a.rows, &m))
+        return rc;
+    a.u = static_cast<const double*>(u);
+    a.temperatures = static_cast<const double*>(t);
+    a.top_ks = static_cast<const int32_t*>(k);
+    a.top_ps = static_cast<const double*>(p);
+    a.min_ps = static_cast<const double*>(m);
+    const int64_t need = cnh_sample_tokens_workspace(&a);
+    if (need < 0)
+        return (int)need;
+    XArray* out;
+    if (int rc = seq_result(ex, q->out, 1, CNH_I32, &a.rows, &out))
+        return rc;
+    a.out = static_cast<int32_t*>(out->slab);
+    if (ex->trace_on) ex->log("sample_tokens " + std::to_string(q->logits.name) + " -> " + std::to_string(q->out) + " rows=" + std::to_string(a.rows));
+    const size_t bytes = ((size_t)need + 255) & ~(size_t)255;
+    if (bytes) {
+        if (int rc = slab_alloc(ex, bytes, false, &a.workspace))
+            return seq_end(ex, rc, q->out);
+        a.workspace_bytes = need;
+    }
+    const int rc = ex->dry ? 0 : cnh_sample_tokens(&a, ex->stream);
+    if (bytes)
+        slab_release(ex, bytes, a.workspace);
+    return seq_end(ex, rc, q->out);
 }
 
 int cnx_sync(cnx_executor* ex) {

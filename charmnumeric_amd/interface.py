@@ -12,6 +12,11 @@ from . import _lib as L
 from . import lazy
 
 
+# calls of the sequence operators: the payload is the structure of their arguments
+_SEQUENCE = {"rms_norm": L.lib.cnx_rms_norm, "short_convolution": L.lib.cnx_short_convolution,
+             "state_scan": L.lib.cnx_state_scan, "sample_tokens": L.lib.cnx_sample_tokens}
+
+
 class CharmNumericInterface:
     def __init__(self, device=0, max_pes=1):
         """device < 0 selects the executor's dry mode: every decision is taken and logged, nothing
@@ -161,6 +166,8 @@ class CharmNumericInterface:
             L.check(L.lib.cnx_fill_uniform(ex, instr.name, seed, stream, lo, hi))
         elif instr.opcode == "fill_cg_matrix":
             L.check(L.lib.cnx_fill_cg_matrix(ex, instr.name, instr.payload[0]))
+        elif instr.opcode in _SEQUENCE:
+            L.check(_SEQUENCE[instr.opcode](ex, C.byref(instr.payload)))
         else:
             raise AssertionError(instr.opcode)
 

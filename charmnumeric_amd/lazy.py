@@ -32,13 +32,14 @@ _ELEMENTWISE = {L.OP_ADD, L.OP_SUB, L.OP_MUL, L.OP_DIV, L.OP_TANH, L.OP_EXP, L.O
 
 
 class Call:
-    """A call that goes to the executor directly, in program order: a bulk upload or a fill."""
+    """A call that goes to the executor directly, in program order: a bulk upload, a fill or a sequence
+    operator."""
 
     __slots__ = ("name", "opcode", "dtype", "payload")
 
     def __init__(self, name, opcode, dtype, payload):
         self.name = name
-        self.opcode = opcode          # "put" | "fill_uniform" | "fill_cg_matrix"
+        self.opcode = opcode          # "put" | "fill_uniform" | "fill_cg_matrix" | a sequence operator
         self.dtype = dtype
         self.payload = payload
 

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 from . import lazy
 from .array import create_array
+from .sequence import sample_tokens  # noqa: F401  (a draw from logits with given random numbers)
 
 
 def randn(*args):

@@ -47,6 +47,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "cnhip.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -169,6 +171,48 @@ int cnx_get(cnx_executor* ex, int ndims, int epoch, int name, int64_t size, int 
 int cnx_put(cnx_executor* ex, int name, int64_t size, int dtype, const void* host_in);
 /* array[i] = lo + (hi-lo)*u01(seed, stream_id, i), i = global row-major index; fp64 arrays. */
 int cnx_fill_uniform(cnx_executor* ex, int name, uint64_t seed, uint64_t stream_id, double lo, double hi);
+/* Operators of recurrent sequence models on whole arrays or unit-step regions of them (cnhip.h:
+ * cnh_rms_norm, cnh_short_convolution, cnh_state_scan, cnh_sample_tokens, with what each computes). Each
+ * runs in program order behind everything received so far, makes one new array (y, out) and leaves it
+ * and every operand stored as one row-major block. Array names of 0 stand for an operand that is not
+ * there. Arrays of one call share one floating-point type except where another is named. */
+typedef struct cnx_operand {
+    int32_t name;
+    cnh_region region;   /* is_global = 1: the whole array */
+} cnx_operand;
+/* x of any rank, the norm along its last dimension; residual: x's extents, receives x + residual. */
+typedef struct cnx_rms_norm_args {
+    cnx_operand x;
+    int32_t residual, weight, y;
+    double eps;
+} cnx_rms_norm_args;
+int cnx_rms_norm(cnx_executor* ex, const cnx_rms_norm_args* args);
+/* x (batch, length, channels), or (batch, channels) for one token per sequence; weight (taps, channels),
+ * bias (channels), state (batch, taps - 1, channels; updated), lengths int32 (batch). */
+typedef struct cnx_short_convolution_args {
+    cnx_operand x;
+    int32_t weight, bias, state, lengths, y;
+    int32_t activation;
+} cnx_short_convolution_args;
+int cnx_short_convolution(cnx_executor* ex, const cnx_short_convolution_args* args);
+/* x, delta, z like the convolution's x; B, C (batch, length, states) or (batch, states); A (channels,
+ * states), skip and delta_bias (channels), state (batch, channels, states; updated), lengths int32 (batch). */
+typedef struct cnx_state_scan_args {
+    cnx_operand x, delta, z, B, C;
+    int32_t A, skip, delta_bias, state, lengths, y;
+    int32_t softplus;
+} cnx_state_scan_args;
+int cnx_state_scan(cnx_executor* ex, const cnx_state_scan_args* args);
+/* logits (rows, vocab) or (vocab); u fp64 (rows); temperatures, top_ps, min_ps fp64 (rows) and top_ks
+ * int32 (rows) where not 0 instead of the scalars; out: int32 (rows). */
+typedef struct cnx_sample_tokens_args {
+    cnx_operand logits;
+    int32_t u, temperatures, top_ks, top_ps, min_ps, out;
+    int32_t top_k;
+    double temperature, top_p, min_p;
+} cnx_sample_tokens_args;
+int cnx_sample_tokens(cnx_executor* ex, const cnx_sample_tokens_args* args);
+
 /* Waits for everything queued so far. */
 int cnx_sync(cnx_executor* ex);
 
