@@ -5,8 +5,13 @@
 //
 // Every cut keeps a prefix of the descending order, so a row needs no full sort: a histogram over the
 // depth (max - l) / temperature finds the bin a cut or the draw falls into, and only that bin (or, when
-// they are few, everything down to the cut) is gathered into shared memory and sorted. A bin that is too
-// crowded for that is split by the bits of its values until it is small enough or one value.
+// they are few, everything down to the cut) is gathered into shared memory and sorted there, by buckets
+// and by counting inside a bucket. A bin that is too crowded for that is split by the bits of its values
+// until it is small enough or one value.
+//
+// A small top-k needs no histogram of the row: the k-th largest of the lanes' own maxima, which the pass
+// for the maximum has left behind, is at most the k-th largest word, so what is not below it (its bin)
+// holds all that top-k keeps and little else. Two passes over the row, no exponential outside the list.
 //
 // Masses are 64-bit integers, w in steps of 2^-45 (coarser beyond 2^17 words, so that a row's sum fits
 // 62 bits): additions in any order give the same sum, so the histogram's atomics cannot change a result.
@@ -18,12 +23,13 @@
 #include "sequence.h"
 
 #include <algorithm>
+#include <limits>
 
 using namespace cnh;
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 2048, kList = 2048;
+constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 2048, kList = kThreads;
 constexpr double kDepth = 32.0, kBinsPerUnit = kBins / kDepth;
 
 template <typename T>
@@ -71,22 +77,22 @@ __device__ __forceinline__ double value_of(uint64_t k) {
     return __longlong_as_double((long long)(k >> 63 ? k & ~(1ull << 63) : ~k));
 }
 
-template <typename V>
-__device__ __forceinline__ V shuffle_up(V v, int o) {
-    return __shfl_up(v, o, 64);
-}
-
 template <typename T>
 struct Shared {
     typedef typename KeyOf<T>::type Key;
     // the first histogram, as running sums including the bin itself once it is complete
-    uint32_t count[kBins];
-    unsigned long long mass[kBins];
+    // (bin kBins takes what lies beyond, with no mass)
+    uint32_t count[kBins + 2];
+    unsigned long long mass[kBins + 2];
+    double level[kBins + 2]; // e^-(bin's depth)
     union {
         struct {
             Key key[kList];
             uint32_t index[kList];
             unsigned long long mass[kList];
+            Key grouped_key[kList];
+            uint32_t grouped_index[kList];
+            uint32_t start[kList + 1]; // of each bucket
         } list;
         struct {
             uint32_t count[kBins];
@@ -95,86 +101,163 @@ struct Shared {
     };
     unsigned long long wave_mass[kWaves];
     uint32_t wave_count[kWaves];
-    Key wave_key[kWaves];
-    uint32_t wave_index[kWaves];
-    unsigned long long found_mass, found_before;
-    uint32_t found, listed, found_count;
+    T wave_top[kWaves];
+    uint32_t found, listed;
+    Key low, high;
+};
+
+// What ends a run of the descending order: a number of words, a mass reached, or a mass passed.
+struct Until {
+    enum Kind { COUNT, REACHED, PASSED } kind;
+    uint32_t words;
+    double reached;
+    unsigned long long passed;
+    __device__ __forceinline__ bool operator()(uint32_t count, unsigned long long mass) const {
+        return kind == COUNT ? count >= words : kind == REACHED ? (double)mass >= reached : mass > passed;
+    }
+};
+
+// Which words a list takes: those of bins b0 to b1 and of bin b2, or (keyed) those with keys low to high.
+template <typename Key>
+struct Range {
+    uint32_t b0, b1, b2;
+    bool keyed;
     Key low, high;
 };
 
 // One row's walk in descending order; all lanes of the workgroup go through it together.
-template <typename T, int VEC>
+template <typename T>
 struct Row {
     typedef typename KeyOf<T>::type Key;
     Shared<T>& sh;
     const T* logits;
     int64_t vocab;
-    double top, inv; // largest logit, 1 / temperature
+    double top, inv; // largest logit (finite), 1 / temperature
     double scale;
     int tid;
 
-    __device__ __forceinline__ double depth(T l) const { return (double)l == top ? 0.0 : (top - (double)l) * inv; }
-    __device__ __forceinline__ int bin_at(double d) const {
-        return d < kDepth ? (int)(d * kBinsPerUnit) : kBins; // NaN: beyond the last bin as well
+    __device__ __forceinline__ void set(T largest, double temperature) {
+        top = (double)largest;
+        inv = fmin(1.0 / temperature, std::numeric_limits<double>::max());
     }
-    __device__ __forceinline__ double weight(double d) const { return exp(-d); }
+    // (max - l) / temperature; no number for NaN
+    __device__ __forceinline__ double depth(T l) const { return (top - (double)l) * inv; }
+    // The nearest bin (bin b is at depth b / kBinsPerUnit), kBins for what is deeper than the last and
+    // for NaN. Adding 1.5 x 2^52 leaves the rounded integer in the low bits of the sum. Every step is
+    // monotone, so bins are.
+    __device__ __forceinline__ static int bin_at(double d, double* rest = nullptr) {
+        const double t = fma(d, kBinsPerUnit, 0x1.8p52);
+        if (rest)
+            *rest = fma(t - 0x1.8p52, -1.0 / kBinsPerUnit, d);
+        return d <= (kBins - 1) / kBinsPerUnit ? __double2loint(t) : kBins;
+    }
+    __device__ __forceinline__ int bin_of(T l) const { return bin_at(depth(l)); }
+    // Logits that the words of bin b0 to b1 lie between, with some room: what a pass tests first.
+    struct Between {
+        T low, high;
+        __device__ __forceinline__ bool has(T l) const { return l >= low && l <= high; }
+    };
+    __device__ __forceinline__ Between between(uint32_t b0, uint32_t b1) const {
+        const double room = 16.0 * (double)std::numeric_limits<T>::epsilon(), step = 1.0 / kBinsPerUnit / inv;
+        const double far = (b1 + 0.5) * step, near = (b0 - 0.5) * step;
+        return {(T)(top - (far + fabs(top)) * room - far),
+                b0 == 0 ? std::numeric_limits<T>::infinity() : (T)(top + (far + fabs(top)) * room - near)};
+    }
+    // e^-depth: the level of the bin times e^-r of the rest, |r| <= 2^-7 (r^6 / 6! is 2^-51 of it).
+    __device__ __forceinline__ double weight_at(int bin, double r) const {
+        double e = -1.0 / 120;
+        e = fma(e, r, 1.0 / 24);
+        e = fma(e, r, -1.0 / 6);
+        e = fma(e, r, 0.5);
+        e = fma(e, r, -1.0);
+        e = fma(e, r, 1.0);
+        return e * sh.level[bin];
+    }
+    __device__ __forceinline__ double weight(T l) const {
+        double r;
+        const int bin = bin_at(depth(l), &r);
+        return bin < kBins ? weight_at(bin, r) : 0.0;
+    }
+    // w * scale below 2^52: adding 2^52 leaves the rounded integer in the low bits
     __device__ __forceinline__ unsigned long long mass_of(double w) const {
-        return (unsigned long long)(w * scale + 0.5);
+        return (unsigned long long)__double_as_longlong(fma(w, scale, 0x1p52)) & 0xfffffffffffffull;
     }
 
-    // f(logit, index) for every word; each lane meets its words in ascending order.
+    // f(pack, index of its first word) for every word: 16-byte packs from the first aligned one on, AHEAD
+    // of a lane at once, and what is before the first and behind the last whole one as packs of one.
     template <typename F>
     __device__ __forceinline__ void sweep(F f) const {
-        constexpr int AHEAD = 4;
-        const int64_t packs = vocab / VEC;
-        for (int64_t i0 = tid; i0 < packs; i0 += (int64_t)kThreads * AHEAD) {
+        constexpr int VEC = Wide<T>::n, AHEAD = 4;
+        const uint32_t words = (uint32_t)vocab;
+        const uint32_t head = min((uint32_t)((16 - ((uintptr_t)logits & 15)) & 15) / (uint32_t)sizeof(T), words);
+        const uint32_t packs = (words - head) / VEC;
+        const T* base = logits + head;
+        uint32_t i0 = 0;
+        for (; i0 + AHEAD * kThreads <= packs; i0 += AHEAD * kThreads) {
             Pack<T, VEC> q[AHEAD];
 #pragma unroll
             for (int a = 0; a < AHEAD; ++a)
-                if (i0 + a * kThreads < packs)
-                    load_pack(q[a], logits + (i0 + a * kThreads) * VEC);
+                load_pack(q[a], base + (int64_t)(i0 + a * kThreads + tid) * VEC);
 #pragma unroll
             for (int a = 0; a < AHEAD; ++a)
-                if (i0 + a * kThreads < packs) {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                        f(q[a].v[j], (uint32_t)((i0 + a * kThreads) * VEC + j));
-                }
+                f(q[a], head + (i0 + a * kThreads + tid) * VEC);
         }
-        if (VEC > 1)
-            for (int64_t i = packs * VEC + tid; i < vocab; i += kThreads)
-                f(logits[i], (uint32_t)i);
+        for (uint32_t i = i0 + tid; i < packs; i += kThreads) {
+            Pack<T, VEC> q;
+            load_pack(q, base + (int64_t)i * VEC);
+            f(q, head + i * VEC);
+        }
+        const uint32_t tail = head + packs * VEC, single = head + (words - tail); // at most 2 (VEC - 1)
+        if ((uint32_t)tid < single) {
+            const uint32_t i = (uint32_t)tid < head ? (uint32_t)tid : tail + ((uint32_t)tid - head);
+            Pack<T, 1> q;
+            q.v[0] = logits[i];
+            f(q, i);
+        }
+    }
+    // f(logit, index) for the words that `test` lets through: in most packs of a row it is none.
+    template <typename P, typename F>
+    __device__ __forceinline__ void sweep_some(P test, F f) const {
+        sweep([&](const auto& q, uint32_t i) {
+            constexpr int N = (int)(sizeof(q.v) / sizeof(T));
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                any |= test(q.v[j]);
+            if (any)
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (test(q.v[j]))
+                        f(q.v[j], i + j);
+        });
     }
 
-    // Turns a histogram into running sums (each bin's own included). Two bins a lane.
-    __device__ __forceinline__ void running_sums(uint32_t* count, unsigned long long* mass) {
-        static_assert(kBins == 2 * kThreads, "two bins a lane");
-        uint32_t c0 = count[2 * tid], c = c0 + count[2 * tid + 1];
-        unsigned long long m0 = mass[2 * tid], m = m0 + mass[2 * tid + 1];
-        const uint32_t c_own = c;
-        const unsigned long long m_own = m;
+    // Sum of v over the lanes up to this one, of the whole workgroup.
+    template <typename V>
+    __device__ __forceinline__ V running_sum(V v, V* waves) const {
         const int lane = tid & 63;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t cu = shuffle_up(c, o);
-            const unsigned long long mu = shuffle_up(m, o);
-            if (lane >= o) {
-                c += cu;
-                m += mu;
-            }
+            const V up = __shfl_up(v, o, 64);
+            if (lane >= o)
+                v += up;
         }
-        if (lane == 63) {
-            sh.wave_count[tid >> 6] = c;
-            sh.wave_mass[tid >> 6] = m;
-        }
+        if (lane == 63)
+            waves[tid >> 6] = v;
         __syncthreads();
-        for (int w = 0; w < tid >> 6; ++w) {
-            c += sh.wave_count[w];
-            m += sh.wave_mass[w];
-        }
-        count[2 * tid] = c - c_own + c0;
+#pragma unroll
+        for (int w = 0; w < kWaves - 1; ++w)
+            v += w < tid >> 6 ? waves[w] : V(0);
+        return v;
+    }
+    // Turns a histogram into running sums (each bin's own included). Two bins a lane.
+    __device__ __forceinline__ void running_sums(uint32_t* count, unsigned long long* mass) {
+        static_assert(kBins == 2 * kThreads, "two bins a lane");
+        const uint32_t c1 = count[2 * tid + 1], c = running_sum(count[2 * tid] + c1, sh.wave_count);
+        const unsigned long long m1 = mass[2 * tid + 1], m = running_sum(mass[2 * tid] + m1, sh.wave_mass);
+        count[2 * tid] = c - c1;
         count[2 * tid + 1] = c;
-        mass[2 * tid] = m - m_own + m0;
+        mass[2 * tid] = m - m1;
         mass[2 * tid + 1] = m;
         __syncthreads();
     }
@@ -203,205 +286,192 @@ struct Row {
         __syncthreads();
     }
 
-    // Words accepted by `take(logit)` into the list, in descending order (ties: ascending index) with
-    // running masses. Returns how many; the caller knows that they fit.
-    template <typename P>
-    __device__ __forceinline__ uint32_t gather(P take) {
+    // The words of a range into the list, in descending order (ties: ascending index) with running masses.
+    // Returns how many there are; beyond kList the list is of no use.
+    __device__ __forceinline__ uint32_t gather(const Range<Key>& g) {
+        sh.list.start[tid] = 0;
         if (tid == 0)
             sh.listed = 0;
         __syncthreads();
-        sweep([&](T l, uint32_t i) {
-            if (take(l)) {
-                const uint32_t at = atomicAdd(&sh.listed, 1u);
-                if (at < kList) {
-                    sh.list.key[at] = key_of(l);
-                    sh.list.index[at] = i;
-                }
+        auto put = [&](T l, uint32_t i) {
+            const uint32_t at = atomicAdd(&sh.listed, 1u);
+            if (at < kList) {
+                sh.list.key[at] = key_of(l);
+                sh.list.index[at] = i;
             }
-        });
-        __syncthreads();
-        const uint32_t n = min(sh.listed, (uint32_t)kList);
-        uint32_t size = 2;
-        while (size < n)
-            size *= 2;
-        for (uint32_t i = n + tid; i < size; i += kThreads) {
-            sh.list.key[i] = 0;
-            sh.list.index[i] = 0xffffffffu;
-        }
-        __syncthreads();
-        // bitonic sort, one pair a lane
-        for (uint32_t run = 2; run <= size; run *= 2)
-            for (uint32_t step = run / 2; step > 0; step /= 2) {
-                const uint32_t a = 2 * tid - (tid & (step - 1)), b = a + step;
-                if (b < size) {
-                    const Key ka = sh.list.key[a], kb = sh.list.key[b];
-                    const uint32_t ia = sh.list.index[a], ib = sh.list.index[b];
-                    const bool before = ka > kb || (ka == kb && ia < ib);
-                    if (before != ((a & run) == 0)) {
-                        sh.list.key[a] = kb;
-                        sh.list.key[b] = ka;
-                        sh.list.index[a] = ib;
-                        sh.list.index[b] = ia;
-                    }
+        };
+        const Between first = between(g.b0, g.b1), second = between(g.b2, g.b2);
+        auto look = [&](auto maybe) {
+            sweep_some(maybe, [&](T l, uint32_t i) {
+                bool take;
+                if (g.keyed) {
+                    const Key k = key_of(l);
+                    take = k >= g.low && k <= g.high;
+                } else {
+                    const uint32_t b = (uint32_t)bin_of(l);
+                    take = (b >= g.b0 && b <= g.b1) || b == g.b2;
                 }
-                __syncthreads();
-            }
-        // running masses, two words a lane
-        unsigned long long m0 = 0, m = 0;
-        if (2 * tid < n)
-            m0 = m = mass_of(weight(depth(value_of(sh.list.key[2 * tid]))));
-        if (2 * tid + 1 < n)
-            m += mass_of(weight(depth(value_of(sh.list.key[2 * tid + 1]))));
-        const unsigned long long own = m;
-        const int lane = tid & 63;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const unsigned long long mu = shuffle_up(m, o);
-            if (lane >= o)
-                m += mu;
-        }
-        if (lane == 63)
-            sh.wave_mass[tid >> 6] = m;
+                if (take)
+                    put(l, i);
+            });
+        };
+        if (g.b0 == 0 && g.b1 == g.b2) // one comparison tells
+            look([&](T l) { return l >= first.low; });
+        else
+            look([&](T l) { return first.has(l) || second.has(l); });
         __syncthreads();
-        for (int w = 0; w < tid >> 6; ++w)
-            m += sh.wave_mass[w];
-        if (2 * tid < kList) {
-            sh.list.mass[2 * tid] = m - own + m0;
-            sh.list.mass[2 * tid + 1] = m;
+        const uint32_t n = sh.listed;
+        if (n > kList) {
+            __syncthreads();
+            return n;
         }
+        // one word a lane from here on: into its bucket (equal steps of the depth, or of the key), ...
+        const int shift = g.keyed ? max(bits_of(g.high - g.low) - 10, 0) : 0;
+        const double from = g.b0 - 0.5, per = (double)kList / (max(g.b1, g.b2) + 1 - g.b0);
+        const bool own = tid < n;
+        Key key = 0;
+        uint32_t index = 0, group = 0, slot = 0;
+        if (own) {
+            key = sh.list.key[tid];
+            index = sh.list.index[tid];
+            group = g.keyed ? (uint32_t)((g.high - key) >> shift)
+                            : min((uint32_t)fmax((depth(value_of(key)) * kBinsPerUnit - from) * per, 0.0),
+                                  (uint32_t)kList - 1);
+            slot = atomicAdd(&sh.list.start[group], 1u);
+        }
+        __syncthreads();
+        const uint32_t size = sh.list.start[tid];
+        const uint32_t upto = running_sum(size, sh.wave_count); // ends in a barrier behind the loads of `size`
+        sh.list.start[tid] = upto - size;
+        if (tid == kThreads - 1)
+            sh.list.start[kList] = upto;
+        __syncthreads();
+        uint32_t begin = 0, end = 0;
+        if (own) {
+            begin = sh.list.start[group];
+            end = sh.list.start[group + 1];
+            sh.list.grouped_key[begin + slot] = key;
+            sh.list.grouped_index[begin + slot] = index;
+        }
+        __syncthreads();
+        // ... and to its place in it, which the words before it in the order leave free
+        uint32_t place = begin;
+        for (uint32_t q = begin; q < end; ++q) {
+            const Key k = sh.list.grouped_key[q];
+            place += k > key || (k == key && sh.list.grouped_index[q] < index);
+        }
+        if (own) {
+            sh.list.key[place] = key;
+            sh.list.index[place] = index;
+        }
+        __syncthreads();
+        const unsigned long long m = own ? mass_of(weight(value_of(sh.list.key[tid]))) : 0;
+        sh.list.mass[tid] = running_sum(m, sh.wave_mass);
         __syncthreads();
         return n;
     }
 
-    // How many of the first n listed words do not satisfy `done(place, running mass)` (monotone).
+    // How many of the first n listed words come before the first that satisfies `done(place)`.
     template <typename P>
     __device__ __forceinline__ uint32_t listed_before(uint32_t n, P done) {
         if (tid == 0)
             sh.found = n;
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint32_t i = 2 * tid + j;
-            if (i < n && done(i) && (i == 0 || !done(i - 1)))
-                sh.found = i;
-        }
+        if (tid < n && done(tid) && (tid == 0 || !done(tid - 1)))
+            atomicMin(&sh.found, (uint32_t)tid);
         __syncthreads();
         const uint32_t i = sh.found;
         __syncthreads();
         return i;
     }
 
-    // The first word in descending order at whose end `done(count, mass)` holds, found in the completed
-    // first histogram; its running mass, and its index when `want_index`.
-    template <typename P>
-    __device__ __forceinline__ void descend(P done, bool want_index, unsigned long long* mass, uint32_t* index) {
-        const uint32_t b = first_bin(sh.count, sh.mass, done);
-        uint32_t base_count = b ? sh.count[b - 1] : 0;
-        unsigned long long base_mass = b ? sh.mass[b - 1] : 0;
-        uint32_t n = sh.count[b] - base_count;
-        Key high = 0, low = 0;
-        if (n <= kList) {
-            n = gather([&](T l) { return bin_at(depth(l)) == (int)b; });
-        } else {
-            // the range of the crowded bin's values
-            Key hi = 0, lo = ~(Key)0;
-            sweep([&](T l, uint32_t) {
-                if (bin_at(depth(l)) == (int)b) {
-                    const Key k = key_of(l);
-                    hi = k > hi ? k : hi;
-                    lo = k < lo ? k : lo;
-                }
-            });
-            if (tid == 0) {
-                sh.high = 0;
-                sh.low = ~(Key)0;
-            }
-            __syncthreads();
-            if constexpr (sizeof(Key) == 8) {
-                atomicMax((unsigned long long*)&sh.high, (unsigned long long)hi);
-                atomicMin((unsigned long long*)&sh.low, (unsigned long long)lo);
-            } else {
-                atomicMax((uint32_t*)&sh.high, (uint32_t)hi);
-                atomicMin((uint32_t*)&sh.low, (uint32_t)lo);
-            }
-            __syncthreads();
-            high = sh.high;
-            low = sh.low;
-            __syncthreads();
-            while (n > kList && low < high) {
-                int width = 0; // bits of high - low
-                for (Key r = high - low; r; r >>= 1)
-                    ++width;
-                const int shift = width > 11 ? width - 11 : 0;
-                clear(sh.sub.count, sh.sub.mass);
-                sweep([&](T l, uint32_t) {
-                    const Key k = key_of(l);
-                    if (k >= low && k <= high) {
-                        const uint32_t s = (uint32_t)((high - k) >> shift);
-                        atomicAdd(&sh.sub.count[s], 1u);
-                        atomicAdd(&sh.sub.mass[s], mass_of(weight(depth(l))));
-                    }
-                });
-                __syncthreads();
-                running_sums(sh.sub.count, sh.sub.mass);
-                const uint32_t s = first_bin(sh.sub.count, sh.sub.mass, [&](uint32_t c, unsigned long long m) {
-                    return done(base_count + c, base_mass + m);
-                });
-                n = sh.sub.count[s] - (s ? sh.sub.count[s - 1] : 0);
-                if (s) {
-                    base_count += sh.sub.count[s - 1];
-                    base_mass += sh.sub.mass[s - 1];
-                }
-                high -= (Key)s << shift;
-                const Key span = ((Key)1 << shift) - 1;
-                low = high - low > span ? high - span : low;
-                __syncthreads();
-            }
-            if (n > kList) {
-                // words of one value: the place follows from their common mass
-                const unsigned long long each = mass_of(weight(depth(value_of(high))));
-                uint32_t lo_j = 1, hi_j = n;
-                while (lo_j < hi_j) {
-                    const uint32_t mid = lo_j + (hi_j - lo_j) / 2;
-                    if (done(base_count + mid, base_mass + mid * each))
-                        hi_j = mid;
-                    else
-                        lo_j = mid + 1;
-                }
-                *mass = base_mass + lo_j * each;
-                if (want_index)
-                    *index = nth_of_value(high, lo_j);
-                return;
-            }
-            n = gather([&](T l) {
-                const Key k = key_of(l);
-                return k >= low && k <= high;
-            });
+    __device__ __forceinline__ static int bits_of(Key v) {
+        return v == 0 ? 0 : sizeof(Key) == 8 ? 64 - __clzll((unsigned long long)v) : 32 - __clz((int)v);
+    }
+    // Splits a bin that is too crowded for the list by the bits of its values until the part with the
+    // first word at whose end `done` holds fits it, or is a single value. g: the bin, then the part;
+    // count, mass: what is in front of the bin, then of the part. Returns the part's words.
+    __device__ __forceinline__ uint32_t narrow(Range<Key>& g, const Until& done, uint32_t& count, unsigned long long& mass) {
+        const Between near = between(g.b2, g.b2);
+        auto test = [&](T l) { return near.has(l); };
+        if (tid == 0) {
+            sh.high = 0;
+            sh.low = ~(Key)0;
         }
-        const uint32_t i = min(
-            listed_before(n, [&](uint32_t j) { return done(base_count + j + 1, base_mass + sh.list.mass[j]); }), n - 1);
-        *mass = base_mass + sh.list.mass[i];
-        *index = sh.list.index[i];
         __syncthreads();
+        Key high = 0, low = ~(Key)0;
+        sweep_some(test, [&](T l, uint32_t) {
+            if (bin_of(l) == (int)g.b2) {
+                const Key k = key_of(l);
+                high = k > high ? k : high;
+                low = k < low ? k : low;
+            }
+        });
+        if constexpr (sizeof(Key) == 8) {
+            atomicMax((unsigned long long*)&sh.high, (unsigned long long)high);
+            atomicMin((unsigned long long*)&sh.low, (unsigned long long)low);
+        } else {
+            atomicMax((uint32_t*)&sh.high, (uint32_t)high);
+            atomicMin((uint32_t*)&sh.low, (uint32_t)low);
+        }
+        __syncthreads();
+        high = sh.high;
+        low = sh.low;
+        uint32_t n;
+        do {
+            const int shift = max(bits_of(high - low) - 11, 0); // kBins parts
+            clear(sh.sub.count, sh.sub.mass);
+            sweep_some(test, [&](T l, uint32_t) {
+                const Key k = key_of(l);
+                if (k >= low && k <= high) {
+                    const uint32_t s = (uint32_t)((high - k) >> shift);
+                    atomicAdd(&sh.sub.count[s], 1u);
+                    atomicAdd(&sh.sub.mass[s], mass_of(weight(l)));
+                }
+            });
+            __syncthreads();
+            running_sums(sh.sub.count, sh.sub.mass);
+            const uint32_t s = first_bin(sh.sub.count, sh.sub.mass, [&](uint32_t c, unsigned long long m) {
+                return done(count + c, mass + m);
+            });
+            n = sh.sub.count[s] - (s ? sh.sub.count[s - 1] : 0);
+            if (s) {
+                count += sh.sub.count[s - 1];
+                mass += sh.sub.mass[s - 1];
+            }
+            high -= (Key)s << shift;
+            const Key span = ((Key)1 << shift) - 1;
+            low = high - low > span ? high - span : low;
+            __syncthreads();
+        } while (n > kList && low < high);
+        g.keyed = true;
+        g.low = low;
+        g.high = high;
+        return n;
     }
 
-    // Index of the nth word (from 1, in ascending order) whose value has this key.
-    __device__ __forceinline__ uint32_t nth_of_value(Key k, uint32_t nth) {
+    // Index of the nth word (from 1, in ascending order) of this value.
+    __device__ __forceinline__ uint32_t nth_of_value(T value, uint32_t nth) {
         uint32_t seen = 0;
         if (tid == 0)
             sh.found = 0xffffffffu;
         __syncthreads();
+        if (nth == 1) {
+            sweep_some([&](T l) { return l == value; }, [&](T, uint32_t i) { atomicMin(&sh.found, i); });
+            __syncthreads();
+            return sh.found;
+        }
         for (int64_t i0 = 0; i0 < vocab; i0 += kThreads) {
             const int64_t i = i0 + tid;
-            const bool hit = i < vocab && key_of(logits[i]) == k;
+            const bool hit = i < vocab && logits[i] == value;
             const unsigned long long ballot = __ballot(hit);
             if ((tid & 63) == 0)
                 sh.wave_count[tid >> 6] = (uint32_t)__popcll(ballot);
             __syncthreads();
             uint32_t before = seen, all = seen;
+#pragma unroll
             for (int w = 0; w < kWaves; ++w) {
-                if (w < tid >> 6)
-                    before += sh.wave_count[w];
+                before += w < tid >> 6 ? sh.wave_count[w] : 0;
                 all += sh.wave_count[w];
             }
             if (hit && before + (uint32_t)__popcll(ballot & ((1ull << (tid & 63)) - 1)) + 1 == nth)
@@ -415,162 +485,285 @@ struct Row {
         __syncthreads();
         return at;
     }
+
+    // A row whose largest logit is infinite: the words that have it share all the mass. Which of them it is.
+    __device__ __forceinline__ uint32_t among_infinite(T value, int64_t top_k, double top_p, double u) {
+        if (tid == 0)
+            sh.listed = 0;
+        __syncthreads();
+        sweep_some([&](T l) { return l == value; }, [&](T, uint32_t) { atomicAdd(&sh.listed, 1u); });
+        __syncthreads();
+        double n = (double)(top_k > 0 ? min(top_k, (int64_t)sh.listed) : (int64_t)sh.listed);
+        if (top_p < 1.0)
+            n = fmax(ceil(top_p * n), 1.0);
+        u = u > 0.0 ? fmin(u, 1.0) : 0.0;
+        return (uint32_t)fmin(floor(u * n) + 1.0, n);
+    }
 };
 
-template <typename T, int VEC>
+template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams<T> p) {
     typedef typename KeyOf<T>::type Key;
     __shared__ Shared<T> sh;
     const int tid = threadIdx.x;
+    for (int b = tid; b <= kBins; b += kThreads)
+        sh.level[b] = b < kBins ? exp(-b / kBinsPerUnit) : 0.0;
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        Row<T, VEC> r{sh, p.logits + row * p.stride, p.vocab, 0.0, 0.0, p.mass_scale, tid};
+        Row<T> r{sh, p.logits + row * p.stride, p.vocab, 0.0, 0.0, p.mass_scale, tid};
         const double temperature = p.temperatures ? p.temperatures[row] : p.temperature;
         const double top_p = p.top_ps ? p.top_ps[row] : p.top_p;
         double min_p = p.min_ps ? p.min_ps[row] : p.min_p;
         min_p = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
         const int64_t top_k = p.top_ks ? p.top_ks[row] : p.top_k;
+        const double u0 = p.u[row], u = u0 > 0.0 ? fmin(u0, 1.0) : 0.0;
 
-        // the largest logit and the lowest index that has it
-        Key best = 0;
-        uint32_t at = 0xffffffffu;
-        r.sweep([&](T l, uint32_t i) {
-            const Key k = key_of(l);
-            if (k > best || (k == best && i < at)) {
-                best = k;
-                at = i;
-            }
+        // the largest logit; each lane keeps its own
+        const T none = -std::numeric_limits<T>::infinity();
+        T own_top = none;
+        r.sweep([&](const auto& q, uint32_t) {
+#pragma unroll
+            for (int j = 0; j < (int)(sizeof(q.v) / sizeof(T)); ++j)
+                own_top = q.v[j] > own_top ? q.v[j] : own_top; // NaN: never
         });
+        T top = own_top;
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) {
-            const Key k = (Key)__shfl_xor(best, o, 64);
-            const uint32_t i = __shfl_xor(at, o, 64);
-            if (k > best || (k == best && i < at)) {
-                best = k;
-                at = i;
-            }
+            const T other = __shfl_xor(top, o, 64);
+            top = other > top ? other : top;
         }
-        if ((tid & 63) == 0) {
-            sh.wave_key[tid >> 6] = best;
-            sh.wave_index[tid >> 6] = at;
-        }
+        if ((tid & 63) == 0)
+            sh.wave_top[tid >> 6] = top;
         __syncthreads();
-        for (int w = 0; w < kWaves; ++w) {
-            const Key k = sh.wave_key[w];
-            const uint32_t i = sh.wave_index[w];
-            if (k > best || (k == best && i < at)) {
-                best = k;
-                at = i;
-            }
-        }
-        int32_t drawn = (int32_t)at;
-        if (best <= key_of(-std::numeric_limits<T>::infinity())) {
-            drawn = -1; // every word is masked (or no number)
-        } else if (temperature > 0.0 && top_k != 1 && !(top_p <= 0.0)) {
-            r.top = (double)value_of(best);
-            r.inv = fmin(1.0 / temperature, std::numeric_limits<double>::max());
-            const double u0 = p.u[row], u = u0 > 0.0 ? fmin(u0, 1.0) : 0.0;
-            // The cut of a small top-k comes from counts alone, everything it keeps fits the list, and
-            // the words' masses are formed for the listed ones only. Other rows weigh every word.
-            bool weigh = !(top_k > 0 && top_k <= kList / 2);
-            unsigned long long kept_by_min_p = 0, total = 0;
-            uint32_t last = kBins;  // last bin of the list
-            for (;;) {
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+            top = sh.wave_top[w] > top ? sh.wave_top[w] : top;
+
+        int32_t drawn = -1;        // every word is masked (or no number)
+        T value = top;             // where a place among words of one value decides: the value, and which of
+        uint32_t nth = 0;          // them, counted from 1
+        const bool greedy = !(temperature > 0.0 && top_k != 1 && !(top_p <= 0.0));
+        if (top > none && greedy) {
+            nth = 1;
+        } else if (top > std::numeric_limits<T>::max()) {
+            nth = r.among_infinite(top, top_k, top_p, u);
+        } else if (top > none) {
+            r.set(top, temperature);
+            auto target_of = [&](unsigned long long kept) {
+                return min((unsigned long long)(u * (double)kept), kept - 1);
+            };
+            // A small top-k is cut by the lanes' maxima; other rows weigh every word.
+            bool weigh = !(top_k > 0 && top_k <= kThreads / 2);
+            for (bool again = true; again;) {
+                again = false;
                 r.clear(sh.count, sh.mass);
                 unsigned long long own = 0;
                 if (weigh) {
-                    r.sweep([&](T l, uint32_t) {
-                        const double d = r.depth(l);
-                        const int b = r.bin_at(d);
-                        if (b < kBins) {
-                            const double w = r.weight(d);
-                            const unsigned long long m = r.mass_of(w);
-                            atomicAdd(&sh.count[b], 1u);
-                            atomicAdd(&sh.mass[b], m);
-                            own += w >= min_p ? m : 0;
+                    // no branches, so that a pack's words go through the long chains side by side: what is
+                    // out of reach adds nothing to the bin beyond the last
+                    r.sweep([&](const auto& q, uint32_t) {
+                        constexpr int N = (int)(sizeof(q.v) / sizeof(T));
+                        int b[N];
+                        double w[N];
+#pragma unroll
+                        for (int j = 0; j < N; ++j) {
+                            double rest;
+                            b[j] = r.bin_at(r.depth(q.v[j]), &rest);
+                            w[j] = r.weight_at(b[j], rest);
                         }
+#pragma unroll
+                        for (int j = 0; j < N; ++j)
+                            atomicAdd(&sh.mass[b[j]], r.mass_of(w[j]));
+                        if (min_p > 0.0)
+#pragma unroll
+                            for (int j = 0; j < N; ++j)
+                                own += b[j] < kBins && w[j] >= min_p ? r.mass_of(w[j]) : 0;
+                        if (top_k > 0)
+#pragma unroll
+                            for (int j = 0; j < N; ++j)
+                                atomicAdd(&sh.count[b[j]], 1u);
                     });
-                } else {
-                    r.sweep([&](T l, uint32_t) {
-                        const int b = r.bin_at(r.depth(l));
-                        if (b < kBins)
-                            atomicAdd(&sh.count[b], 1u);
-                    });
+                } else if (own_top > none) {
+                    atomicAdd(&sh.count[r.bin_of(own_top)], 1u);
                 }
                 __syncthreads();
+                if (weigh && !(top_k > 0)) {
+                    // nobody counts: a bin's words weigh its level times e^(-1/128) or more, which
+                    // tells how many they are nearly enough to decide whether a list takes them
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int b = 2 * tid + j;
+                        const double each = fmax(sh.level[b] * 0.992 * p.mass_scale, 1.0);
+                        sh.count[b] = (uint32_t)fmin(ceil((double)sh.mass[b] / each), (double)p.vocab);
+                    }
+                }
                 r.running_sums(sh.count, sh.mass);
                 const uint32_t words = sh.count[kBins - 1];
-                total = sh.mass[kBins - 1];
+                const unsigned long long total = sh.mass[kBins - 1];
+                auto count_of = [&](uint32_t b0, uint32_t b1) { return sh.count[b1] - (b0 ? sh.count[b0 - 1] : 0); };
+                Until until{Until::COUNT, (uint32_t)max(top_k, (int64_t)0), top_p * (double)total, 0};
                 uint32_t by_k = kBins, by_p = kBins, by_min_p = kBins;
-                if (top_k > 0 && top_k < (int64_t)words)
-                    by_k = r.first_bin(sh.count, sh.mass, [&](uint32_t c, unsigned long long) { return c >= top_k; });
-                if (weigh && top_p < 1.0) {
-                    const double want = top_p * (double)total;
-                    by_p = r.first_bin(sh.count, sh.mass,
-                                       [&](uint32_t, unsigned long long m) { return (double)m >= want; });
-                }
+                if (top_k > 0 && top_k <= (int64_t)words)
+                    by_k = r.first_bin(sh.count, sh.mass, until);
+                until.kind = Until::REACHED;
+                if (weigh && top_p < 1.0)
+                    by_p = r.first_bin(sh.count, sh.mass, until);
                 if (min_p > 0.0)
                     by_min_p = (uint32_t)fmin(-log(min_p) * kBinsPerUnit + 1.0, (double)kBins); // one to spare
-                last = min(min(by_k, by_p), by_min_p);
+                uint32_t last = min(min(by_k, by_p), by_min_p); // last bin of a list of all that is kept
                 // p of what top-k leaves needs all of that in the list
                 if (top_p < 1.0 && top_k > 0 && (!weigh || by_k != kBins))
                     last = by_k;
                 last = min(last, (uint32_t)kBins - 1);
-                const uint32_t words_listed = sh.count[last];
-                if (weigh) {
-                    // sum of `own` over the workgroup
+                if (weigh && min_p > 0.0) {
+                    // mass of the words that min-p keeps: the sum of `own` over the workgroup
 #pragma unroll
                     for (int o = 32; o >= 1; o >>= 1)
                         own += __shfl_xor(own, o, 64);
                     if ((tid & 63) == 0)
                         sh.wave_mass[tid >> 6] = own;
                     __syncthreads();
-                    kept_by_min_p = 0;
+                    own = 0;
+#pragma unroll
                     for (int w = 0; w < kWaves; ++w)
-                        kept_by_min_p += sh.wave_mass[w];
+                        own += sh.wave_mass[w];
                     __syncthreads();
                 }
-                if (words_listed <= kList) {
-                    const uint32_t n = r.gather([&](T l) { return r.bin_at(r.depth(l)) <= (int)last; });
-                    uint32_t cut = top_k > 0 ? (uint32_t)min((int64_t)n, top_k) : n;
-                    if (top_p < 1.0) {
-                        // without a top-k that cuts, the list may end before the last word that counts
-                        const unsigned long long of = weigh && by_k == kBins ? total : sh.list.mass[cut - 1];
-                        const double want = top_p * (double)of;
-                        cut = min(cut, r.listed_before(n, [&](uint32_t i) { return (double)sh.list.mass[i] >= want; }) + 1);
+
+                // ALL: everything kept in one list. Otherwise the cuts one by one: by COUNT what top-k
+                // leaves, by MASS what top-p does; DRAW the word. Where top-p's cut is known to a bin the
+                // draw is known to a few: BOTH gathers the words of both.
+                enum { ALL, BY_COUNT, BOTH, BY_MASS, DRAW } stage = ALL;
+                unsigned long long most = total; // mass kept, as far as it is cut
+                Range<Key> g;
+                g.keyed = false;
+                uint32_t base_count = 0;
+                unsigned long long base_mass = 0;
+                if (weigh && sh.count[last] > kList)
+                    stage = by_k != kBins ? BY_COUNT : BOTH;
+                for (bool more = true; more;) {
+                    uint32_t n = kList + 1;
+                    if (!g.keyed) {
+                        if (stage == ALL) {
+                            g.b0 = 0;
+                            g.b1 = g.b2 = last;
+                            n = 0; // tried whatever the counts say: they may be those of the lanes' maxima
+                        } else if (stage == BOTH) {
+                            until.kind = Until::REACHED;
+                            const uint32_t cut = top_p < 1.0 ? r.first_bin(sh.count, sh.mass, until) : kBins;
+                            if (min_p > 0.0)
+                                most = min(most, own);
+                            if (cut == kBins || (cut ? sh.mass[cut - 1] : 0) >= most) {
+                                stage = DRAW; // top-p takes nothing away
+                                continue;
+                            }
+                            base_mass = cut ? sh.mass[cut - 1] : 0;
+                            until.kind = Until::PASSED;
+                            until.passed = target_of(max(base_mass, 1ull));
+                            g.b0 = r.first_bin(sh.count, sh.mass, until);
+                            until.passed = target_of(min(most, sh.mass[cut]));
+                            g.b1 = r.first_bin(sh.count, sh.mass, until);
+                            g.b2 = cut;
+                            n = count_of(g.b0, g.b1) + count_of(cut, cut);
+                        } else {
+                            until.kind = stage == BY_COUNT ? Until::COUNT : stage == BY_MASS ? Until::REACHED : Until::PASSED;
+                            until.passed = target_of(most);
+                            g.b0 = g.b1 = g.b2 = r.first_bin(sh.count, sh.mass, until);
+                            base_count = g.b2 ? sh.count[g.b2 - 1] : 0;
+                            base_mass = g.b2 ? sh.mass[g.b2 - 1] : 0;
+                            n = count_of(g.b2, g.b2);
+                        }
+                    } else {
+                        n = 0; // narrowed to what fits
                     }
-                    if (min_p > 0.0)
-                        cut = min(cut, r.listed_before(n, [&](uint32_t i) {
-                            return !(r.weight(r.depth(value_of(sh.list.key[i]))) >= min_p);
-                        }));
-                    const unsigned long long kept = sh.list.mass[cut - 1];
-                    const unsigned long long target = min((unsigned long long)(u * (double)kept), kept - 1);
-                    const uint32_t i =
-                        r.listed_before(cut, [&](uint32_t j) { return sh.list.mass[j] > target; });
-                    drawn = (int32_t)sh.list.index[min(i, cut - 1)];
-                    break;
-                }
-                if (weigh) {
+                    if (n <= kList)
+                        n = r.gather(g);
+                    unsigned long long at = 0; // running mass at the word looked for
                     uint32_t index = 0;
-                    unsigned long long of = total;
-                    if (by_k != kBins)
-                        r.descend([&](uint32_t c, unsigned long long) { return c >= top_k; }, false, &of, &index);
-                    unsigned long long kept = of;
-                    if (top_p < 1.0) {
-                        const double want = top_p * (double)of;
-                        r.descend([&](uint32_t, unsigned long long m) { return (double)m >= want; }, false, &kept,
-                                  &index);
-                        kept = min(kept, of);
+                    if (n > kList) {
+                        if (stage == ALL) {
+                            if (!weigh) { // a crowd at the cut: weigh every word
+                                weigh = again = true;
+                                break;
+                            }
+                            stage = by_k != kBins ? BY_COUNT : BOTH;
+                            continue;
+                        }
+                        if (stage == BOTH) {
+                            stage = BY_MASS;
+                            continue;
+                        }
+                        n = r.narrow(g, until, base_count, base_mass);
+                        if (n <= kList)
+                            continue;
+                        // words of one value: the place follows from their common mass
+                        value = value_of(g.high);
+                        const unsigned long long each = r.mass_of(r.weight(value));
+                        uint32_t lo = 1, hi = n;
+                        while (lo < hi) {
+                            const uint32_t mid = lo + (hi - lo) / 2;
+                            if (until(base_count + mid, base_mass + mid * each))
+                                hi = mid;
+                            else
+                                lo = mid + 1;
+                        }
+                        at = base_mass + lo * each;
+                        if (stage == DRAW)
+                            nth = lo;
+                    } else if (stage == ALL) {
+                        uint32_t cut = top_k > 0 ? (uint32_t)min((int64_t)n, top_k) : n;
+                        if (top_p < 1.0) {
+                            // without a top-k that cuts, the list may end before the last word that counts
+                            const double want = top_p * (double)(weigh && by_k == kBins ? total : sh.list.mass[cut - 1]);
+                            cut = min(cut, r.listed_before(n, [&](uint32_t i) { return (double)sh.list.mass[i] >= want; }) + 1);
+                        }
+                        if (min_p > 0.0)
+                            cut = min(cut, r.listed_before(n, [&](uint32_t i) {
+                                return !(r.weight(value_of(sh.list.key[i])) >= min_p);
+                            }));
+                        const unsigned long long target = target_of(sh.list.mass[cut - 1]);
+                        const uint32_t i = r.listed_before(cut, [&](uint32_t j) { return sh.list.mass[j] > target; });
+                        drawn = (int32_t)sh.list.index[min(i, cut - 1)];
+                        break;
+                    } else if (stage == BOTH) {
+                        // running masses of the row: whole bins stand in the list, with a gap behind b1
+                        const uint32_t head = g.b1 >= g.b2 ? n : r.listed_before(n, [&](uint32_t i) {
+                            return r.bin_of(value_of(sh.list.key[i])) > (int)g.b1;
+                        });
+                        const unsigned long long base = g.b0 ? sh.mass[g.b0 - 1] : 0;
+                        const unsigned long long skipped = head < n ? base_mass - sh.list.mass[head - 1] : 0;
+                        auto upto = [&](uint32_t i) { return sh.list.mass[i] + (i < head ? base : skipped); };
+                        const uint32_t end = min(r.listed_before(n, [&](uint32_t i) { return (double)upto(i) >= until.reached; }), n - 1);
+                        const unsigned long long target = target_of(min(most, upto(end)));
+                        const uint32_t i = r.listed_before(n, [&](uint32_t j) { return upto(j) > target; });
+                        drawn = (int32_t)sh.list.index[min(i, n - 1)];
+                        break;
+                    } else {
+                        const uint32_t i = min(r.listed_before(n, [&](uint32_t j) {
+                            return until(base_count + j + 1, base_mass + sh.list.mass[j]);
+                        }), n - 1);
+                        at = base_mass + sh.list.mass[i];
+                        index = sh.list.index[i];
+                        __syncthreads();
                     }
-                    if (min_p > 0.0)
-                        kept = min(kept, kept_by_min_p);
-                    const unsigned long long target = min((unsigned long long)(u * (double)kept), kept - 1);
-                    r.descend([&](uint32_t, unsigned long long m) { return m > target; }, true, &kept, &index);
-                    drawn = (int32_t)index;
-                    break;
+                    // one cut further
+                    g.keyed = false;
+                    if (stage == BY_COUNT) {
+                        most = at;
+                        until.reached = top_p * (double)most;
+                        stage = BOTH;
+                    } else if (stage == BY_MASS) {
+                        most = min(most, at);
+                        stage = DRAW;
+                    } else {
+                        drawn = (int32_t)index;
+                        more = false;
+                    }
                 }
-                weigh = true; // a crowd at the cut: weigh every word and walk down to it
             }
         }
+        __syncthreads();
+        if (nth)
+            drawn = (int32_t)r.nth_of_value(value, nth);
         if (tid == 0)
             p.out[row] = drawn;
         __syncthreads(); // the next row writes the shared memory again
@@ -598,12 +791,7 @@ int run(const cnh_sample_tokens_args* a, hipStream_t st) {
     while (((int64_t)1 << bits) < a->vocab)
         ++bits;
     p.mass_scale = (double)((uint64_t)1 << std::min(45, 62 - bits));
-    constexpr int W = Wide<T>::n;
-    const unsigned groups = (unsigned)std::min<int64_t>(p.rows, 1 << 20);
-    if (aligned_to(p.logits, 16) && (p.rows == 1 || p.stride % W == 0))
-        sample_kernel<T, W><<<groups, kThreads, 0, st>>>(p);
-    else
-        sample_kernel<T, 1><<<groups, kThreads, 0, st>>>(p);
+    sample_kernel<T><<<(unsigned)std::min<int64_t>(p.rows, 1 << 20), kThreads, 0, st>>>(p);
     CNH_HIP(hipGetLastError());
     return 0;
 }
