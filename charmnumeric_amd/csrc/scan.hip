@@ -32,16 +32,19 @@ struct ScanParams {
     int64_t first_batch; // of this launch
     int states, softplus;
     const T *x, *delta, *z;
-    int64_t x_bs, x_s, delta_bs, delta_s, z_bs, z_s;
+    int64_t x_bs, delta_bs, z_bs; // elements between sequences
+    uint32_t x_s, delta_s, z_s;   // bytes between tokens: half the scalar registers of a 64-bit stride
     const T* A;
     const T *B, *C;
-    int64_t B_bs, B_s, C_bs, C_s;
+    int64_t B_bs, C_bs;
+    uint32_t B_s, C_s;
     const T *skip, *delta_bias;
     const T* state_in;
     T* state_out;
     const int32_t* lengths;
     T* y;
-    int64_t y_bs, y_s;
+    int64_t y_bs;
+    uint32_t y_s;
     int64_t piece;  // tokens per piece (a single token: sequences per workgroup)
     int pieces;     // 1: no cut
     T* carry;       // [batch][pieces][states][channels]: the state a piece leaves, then the one it starts from
@@ -101,9 +104,41 @@ __device__ __forceinline__ T& at(T* row, uint32_t bytes) {
     return *reinterpret_cast<T*>(reinterpret_cast<char*>(row) + bytes);
 }
 
+// v of lane U of every G neighbouring ones (G 2 or 4), in all of them.
+template <int G, int U, typename T>
+__device__ __forceinline__ T from_lane(T v) {
+    return partner<G == 4 ? U * 0x55 : U ? 0xF5 : 0xA0>(v);
+}
+
+// A row so many bytes further.
+template <typename T>
+__device__ __forceinline__ const T* on(const T* row, int64_t bytes) {
+    return reinterpret_cast<const T*>(reinterpret_cast<const char*>(row) + bytes);
+}
+template <typename T>
+__device__ __forceinline__ T* on(T* row, int64_t bytes) {
+    return reinterpret_cast<T*>(reinterpret_cast<char*>(row) + bytes);
+}
+
 // Memory that no kernel in flight writes, for loads at addresses the whole wavefront shares.
 template <typename T>
 using Uniform = const __attribute__((address_space(4))) T;
+
+// A row of B or C in scalar registers: BYTES of them, from an address aligned to 4.
+template <int BYTES>
+struct ScalarRow;
+template <>
+struct ScalarRow<16> {
+    typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <>
+struct ScalarRow<32> {
+    typedef uint32_t type __attribute__((ext_vector_type(8), aligned(4)));
+};
+template <>
+struct ScalarRow<64> {
+    typedef uint32_t type __attribute__((ext_vector_type(16), aligned(4)));
+};
 
 // NPL states (n0 .. n0 + NPL) of one token's B or C. FULL: all of them exist, the rows of A and of the
 // states are aligned for wide accesses and, with S > 1, those of B and C too.
@@ -112,8 +147,10 @@ __device__ __forceinline__ void load_states(T (&v)[NPL], const T* row, int n0, i
     if constexpr (S == 1) {
         Uniform<T>* u = (Uniform<T>*)(uintptr_t)row;
 #pragma unroll
-        for (int i = 0; i < NPL; ++i)
-            v[i] = FULL ? u[i] : i < states ? u[i] : T(0);
+        for (int i = 0; i < NPL; ++i) {
+            const T at = u[FULL ? i : min(i, states - 1)];
+            v[i] = FULL || i < states ? at : T(0);
+        }
     } else if constexpr (FULL) {
         Pack<T, NPL> q;
         load_pack(q, row + n0);
@@ -121,9 +158,12 @@ __device__ __forceinline__ void load_states(T (&v)[NPL], const T* row, int n0, i
         for (int i = 0; i < NPL; ++i)
             v[i] = q.v[i];
     } else {
+        // the last state again for those that do not exist: no branches between the loads
 #pragma unroll
-        for (int i = 0; i < NPL; ++i)
-            v[i] = n0 + i < states ? row[n0 + i] : T(0);
+        for (int i = 0; i < NPL; ++i) {
+            const T at = row[min(n0 + i, states - 1)];
+            v[i] = n0 + i < states ? at : T(0);
+        }
     }
 }
 
@@ -180,7 +220,7 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
     const T* zp = p.z ? p.z + b * p.z_bs : nullptr;
     // without a gate the loads of z repeat those of x: cheaper than a branch around each
     const T* zq = zp ? zp : xp;
-    const int64_t zq_s = zp ? p.z_s : p.x_s;
+    const uint32_t zq_s = zp ? p.z_s : p.x_s;
     T* yp = p.y + b * p.y_bs;
     T* slot = p.carry + ((b * p.pieces + piece) * p.states + n0) * p.channels + d;
     Pack<T, NPL> h = {};
@@ -195,67 +235,145 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
     }
     T steps = 0;
     // M tokens from t0 on; their steps and gates first, so that the branches on what the call has come once
-    const T *Bt_row = p.B + b * p.B_bs + begin * p.B_s, *Ct_row = p.C + b * p.C_bs + begin * p.C_s;
-    T* y_row = yp + begin * p.y_s;
+    const T *Bt_row = on(p.B + b * p.B_bs, begin * (int64_t)p.B_s),
+            *Ct_row = on(p.C + b * p.C_bs, begin * (int64_t)p.C_s);
+    T* y_row = on(yp, begin * (int64_t)p.y_s);
+    // B and C one token ahead in scalar registers, where two tokens' rows of both fit them.
+    constexpr bool EARLY = S == 1 && FULL && NPL * sizeof(T) <= 64;
+    typedef typename ScalarRow<EARLY ? NPL * sizeof(T) : 16>::type Scalars;
+    Scalars B_early = {}, C_early = {};
+    int left = end > begin ? (int)(end - begin) : 0; // rows not sent for yet
+    auto send = [&]() { // behind the last row that one again
+        B_early = *(Uniform<Scalars>*)(uintptr_t)Bt_row;
+        if constexpr (!PARTIAL)
+            C_early = *(Uniform<Scalars>*)(uintptr_t)Ct_row;
+        --left;
+        Bt_row = on(Bt_row, left > 0 ? p.B_s : 0);
+        Ct_row = on(Ct_row, left > 0 ? p.C_s : 0);
+    };
+    if constexpr (EARLY)
+        if (left > 0)
+            send();
     auto tokens = [&](auto count, const T* xc, const T* dc, const T* zc) {
         constexpr int M = decltype(count)::value;
-        T s[M], gate[M];
+        // With S > 1 B and C are vector loads: all of the group's before the first is waited for. (Scalar
+        // registers have no room for that.)
+        T Bt[S > 1 ? M : 1][NPL], Ct[S > 1 && !PARTIAL ? M : 1][NPL];
+        if constexpr (S > 1) {
 #pragma unroll
-        for (int u = 0; u < M; ++u)
-            s[u] = dc[u] + bias;
-        if (p.softplus)
-#pragma unroll
-            for (int u = 0; u < M; ++u)
-                s[u] = softplus(s[u]);
-        if (!PARTIAL && zp) {
-#pragma unroll
-            for (int u = 0; u < M; ++u)
-                gate[u] = silu(zc[u]);
+            for (int u = 0; u < M; ++u) {
+                load_states<T, NPL, S, FULL>(Bt[u], on(Bt_row, u * (int64_t)p.B_s), n0, p.states);
+                if constexpr (!PARTIAL)
+                    load_states<T, NPL, S, FULL>(Ct[u], on(Ct_row, u * (int64_t)p.C_s), n0, p.states);
+            }
         }
+        T s[M], gate[M];
+        // The lanes of a channel have its tokens in common: each of G neighbours works out the steps and
+        // gates of M / G tokens and hands them to the others.
+        constexpr int G = M % 4 == 0 && S >= 4 ? 4 : M % 2 == 0 && S >= 2 ? 2 : 1;
+        const int turn = (int)(lane % G);
+        auto shared = [&](const T* in, T* out, auto f) {
+            if constexpr (G == 1) {
+#pragma unroll
+                for (int u = 0; u < M; ++u)
+                    out[u] = f(in[u]);
+            } else {
+#pragma unroll
+                for (int u = 0; u < M; u += G) {
+                    T mine = in[u];
+#pragma unroll
+                    for (int i = 1; i < G; ++i) {
+                        const T other = in[u + i];
+                        mine = turn == i ? other : mine;
+                    }
+                    mine = f(mine);
+                    out[u] = from_lane<G, 0>(mine);
+                    out[u + 1] = from_lane<G, 1>(mine);
+                    if constexpr (G == 4) {
+                        out[u + 2] = from_lane<G, 2>(mine);
+                        out[u + 3] = from_lane<G, 3>(mine);
+                    }
+                }
+            }
+        };
+        if (p.softplus) {
+            shared(dc, s, [&](T v) { return softplus(v + bias); });
+        } else {
+#pragma unroll
+            for (int u = 0; u < M; ++u)
+                s[u] = dc[u] + bias;
+        }
+        if (!PARTIAL && zp)
+            shared(zc, gate, [&](T v) { return silu(v); });
 #pragma unroll
         for (int u = 0; u < M; ++u) {
             const T sx = s[u] * xc[u];
-            T Bt[NPL];
-            load_states<T, NPL, S, FULL>(Bt, Bt_row, n0, p.states);
-            Bt_row += p.B_s;
+            constexpr bool GROUPED = S > 1;
+            T(&B)[NPL] = Bt[GROUPED ? u : 0];
+            if constexpr (EARLY) {
+                // These rows have been on their way since the last token. They are waited for here, the
+                // next token's are sent for, and only then the work begins that covers their flight:
+                // scalar loads return in any order, so a wait further down would wait for both.
+                asm volatile("" : : "s"(B_early));
+                if constexpr (!PARTIAL)
+                    asm volatile("" : : "s"(C_early));
+                __builtin_amdgcn_sched_barrier(0);
+                const Scalars B_now = B_early, C_now = C_early;
+                send();
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_memcpy(B, &B_now, sizeof B);
+                if constexpr (!PARTIAL)
+                    __builtin_memcpy(Ct[0], &C_now, sizeof Ct[0]);
+            } else {
+                if constexpr (!GROUPED)
+                    load_states<T, NPL, S, FULL>(B, Bt_row, n0, p.states);
+                Bt_row = on(Bt_row, p.B_s);
+            }
             if constexpr (PARTIAL) {
                 steps += s[u];
 #pragma unroll
                 for (int i = 0; i < NPL; ++i)
-                    h.v[i] = decay(s[u], rate.v[i]) * h.v[i] + sx * Bt[i];
+                    h.v[i] = decay(s[u], rate.v[i]) * h.v[i] + sx * B[i];
             } else {
-                T Ct[NPL], sum = 0;
-                load_states<T, NPL, S, FULL>(Ct, Ct_row, n0, p.states);
-                Ct_row += p.C_s;
+                T(&C)[NPL] = Ct[GROUPED ? u : 0];
+                if constexpr (!GROUPED && !EARLY)
+                    load_states<T, NPL, S, FULL>(C, Ct_row, n0, p.states);
+                if constexpr (!EARLY)
+                    Ct_row = on(Ct_row, p.C_s);
+                T sum = 0;
 #pragma unroll
                 for (int i = 0; i < NPL; ++i) {
-                    h.v[i] = decay(s[u], rate.v[i]) * h.v[i] + sx * Bt[i];
-                    sum += Ct[i] * h.v[i];
+                    h.v[i] = decay(s[u], rate.v[i]) * h.v[i] + sx * B[i];
+                    sum += C[i] * h.v[i];
                 }
                 sum = lanes_sum<S>(sum) + skip * xc[u];
                 if (zp)
                     sum *= gate[u];
                 if (first && live)
                     at(y_row, off) = sum;
-                y_row += p.y_s;
+                y_row = on(y_row, p.y_s);
             }
         }
     };
     // Whole groups of tokens, the next group's x, delta and z on their way meanwhile, then what is left.
-    // Behind the last group the last one is fetched again: no branch stands between a load and its wait.
-    const T *x_row = xp + begin * p.x_s, *d_row = dp + begin * p.delta_s, *z_row = zq + begin * zq_s;
+    // Behind the last group its last token is fetched again: no branch stands between a load and its wait.
+    const T *x_row = on(xp, begin * (int64_t)p.x_s), *d_row = on(dp, begin * (int64_t)p.delta_s),
+            *z_row = on(zq, begin * (int64_t)zq_s);
     const int groups = end > begin ? (int)((end - begin) / AHEAD) : 0, rest = end > begin ? (int)((end - begin) % AHEAD) : 0;
     if (groups > 0) {
         T xs[AHEAD], ds[AHEAD], zs[AHEAD];
-        auto fetch = [&]() {
+        auto fetch = [&](uint32_t x_on, uint32_t d_on, uint32_t z_on) {
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                xs[u] = at(x_row + u * p.x_s, off);
-                ds[u] = at(d_row + u * p.delta_s, off);
-                zs[u] = PARTIAL ? T(0) : at(z_row + u * zq_s, off);
+                xs[u] = at(x_row, off);
+                ds[u] = at(d_row, off);
+                zs[u] = PARTIAL ? T(0) : at(z_row, off);
+                x_row = on(x_row, x_on);
+                d_row = on(d_row, d_on);
+                z_row = on(z_row, z_on);
             }
         };
-        fetch();
+        fetch(p.x_s, p.delta_s, zq_s);
         for (int g = 1; g <= groups; ++g) {
             T xc[AHEAD], dc[AHEAD], zc[AHEAD];
 #pragma unroll
@@ -264,22 +382,22 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
                 dc[u] = ds[u];
                 zc[u] = zs[u];
             }
-            const int on = g < groups ? AHEAD : 0;
-            x_row += on * p.x_s;
-            d_row += on * p.delta_s;
-            z_row += on * zq_s;
-            fetch();
+            const bool more = g < groups;
+            x_row = on(x_row, more ? 0 : -(int64_t)p.x_s);
+            d_row = on(d_row, more ? 0 : -(int64_t)p.delta_s);
+            z_row = on(z_row, more ? 0 : -(int64_t)zq_s);
+            fetch(more ? p.x_s : 0, more ? p.delta_s : 0, more ? zq_s : 0);
             tokens(std::integral_constant<int, AHEAD>(), xc, dc, zc);
         }
-        x_row += AHEAD * p.x_s;
-        d_row += AHEAD * p.delta_s;
-        z_row += AHEAD * zq_s;
+        x_row = on(x_row, p.x_s);
+        d_row = on(d_row, p.delta_s);
+        z_row = on(z_row, zq_s);
     }
     for (int r = 0; r < rest; ++r) {
         const T xc = at(x_row, off), dc = at(d_row, off), zc = PARTIAL ? T(0) : at(z_row, off);
-        x_row += p.x_s;
-        d_row += p.delta_s;
-        z_row += zq_s;
+        x_row = on(x_row, p.x_s);
+        d_row = on(d_row, p.delta_s);
+        z_row = on(z_row, zq_s);
         tokens(std::integral_constant<int, 1>(), &xc, &dc, &zc);
     }
     if constexpr (PARTIAL) {
@@ -294,7 +412,7 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
     } else {
         if (first && live)
             for (int64_t t = std::max(begin, end); t < stop; ++t)
-                (yp + t * p.y_s)[d] = T(0);
+                at(on(yp, t * (int64_t)p.y_s), off) = T(0);
         if (p.state_out && piece == p.pieces - 1 && live) {
             store_states<T, NPL, FULL>(h, p.state_out + (b * p.channels + d) * p.states, n0, p.states);
         }
@@ -302,16 +420,16 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
 }
 
 // The state each piece starts from, in place of the one it leaves: 64 channels of one state per
-// workgroup, SEGMENTS x GROUP pieces a round. A lane loads its GROUP pieces at once, folds them to one,
+// workgroup, up to kSegments x GROUP pieces a round (as many segments as the pieces need). A lane loads its GROUP pieces at once, folds them to one,
 // takes what the segments before it leave from shared memory and walks its pieces again in registers;
 // one lane per channel that walks all pieces by itself waits for memory once per GROUP of them instead
 // (128 pieces of 2048 x 16 fp32 states: 22.5 us).
-constexpr int kSegments = 8;
+constexpr int kSegments = 8, kGroup = 8;
 template <typename T>
 __global__ __launch_bounds__(64 * kSegments) void carry_kernel(ScanParams<T> p) {
-    constexpr int GROUP = 8;
+    constexpr int GROUP = kGroup;
     __shared__ T left_by[kSegments][64], steps_of[kSegments][64];
-    const int seg = threadIdx.y, lane = threadIdx.x;
+    const int seg = threadIdx.y, lane = threadIdx.x, segments = blockDim.y;
     const int64_t own = (int64_t)blockIdx.x * 64 + lane;
     const bool live = own < p.channels;
     const int64_t d = live ? own : p.channels - 1;
@@ -319,7 +437,7 @@ __global__ __launch_bounds__(64 * kSegments) void carry_kernel(ScanParams<T> p) 
     const int64_t b = p.first_batch + blockIdx.z;
     const T rate = rate_of(p.A[d * p.states + n]);
     T start = p.state_in ? p.state_in[(b * p.channels + d) * p.states + n] : T(0); // of the round
-    for (int c0 = 0; c0 < p.pieces; c0 += kSegments * GROUP) {
+    for (int c0 = 0; c0 < p.pieces; c0 += segments * GROUP) {
         const int c1 = c0 + seg * GROUP;
         T left[GROUP], steps[GROUP];
 #pragma unroll
@@ -340,7 +458,7 @@ __global__ __launch_bounds__(64 * kSegments) void carry_kernel(ScanParams<T> p) 
         __syncthreads();
         T at = start;
         h = start;
-        for (int s = 0; s < kSegments; ++s) {
+        for (int s = 0; s < segments; ++s) {
             if (s == seg)
                 h = at;
             at = decay(steps_of[s][lane], rate) * at + left_by[s][lane];
@@ -442,7 +560,7 @@ Plan plan_of(const cnh_state_scan_args* a) {
     // Few states per lane spread a small call over more lanes and make a single token's states one
     // 16-byte access each; many states per lane share a token's step and gate. Few as long as the
     // pieces of 32 tokens that the call could be cut into would not fill the device with many.
-    const int many = N <= 8 ? 8 : 16;
+    const int many = N <= 8 ? 8 : N <= 16 || N > 32 ? 16 : 32;
     q.npl = many;
     if (N <= 64 && (N <= 4 || L <= 1 || waves(lanes(many)) * std::max<int64_t>(1, L / 32) < 2 * kUnits))
         q.npl = 4;
@@ -455,7 +573,7 @@ Plan plan_of(const cnh_state_scan_args* a) {
         q.piece = std::max<int64_t>(1, (a->batch + slices - 1) / slices);
         q.piece = std::max(q.piece, (a->batch + 65534) / 65535);
     } else {
-        if (w <= 2 * kUnits && w > 0)
+        if (w < 3 * kUnits / 2 && w > 0)
             q.pieces = (int)std::max<int64_t>(1, std::min(4 * kUnits / w, L / 16));
         q.piece = (L + q.pieces - 1) / q.pieces;
         q.pieces = (int)((L + q.piece - 1) / q.piece);
@@ -478,7 +596,8 @@ int launch(ScanParams<T> p, hipStream_t st) {
         const unsigned gz = (unsigned)std::min<int64_t>(p.batch - p.first_batch, 65535);
         if (p.pieces > 1) {
             scan_kernel<T, NPL, S, FULL, true><<<dim3(gx, p.pieces - 1, gz), 64, 0, st>>>(p);
-            carry_kernel<T><<<dim3((unsigned)((p.channels + 63) / 64), p.states, gz), dim3(64, kSegments), 0, st>>>(p);
+            const int segments = std::min(kSegments, (p.pieces + kGroup - 1) / kGroup);
+            carry_kernel<T><<<dim3((unsigned)((p.channels + 63) / 64), p.states, gz), dim3(64, segments), 0, st>>>(p);
         }
         scan_kernel<T, NPL, S, FULL, false><<<dim3(gx, p.pieces, gz), 64, 0, st>>>(p);
     }
@@ -503,18 +622,19 @@ int run(const cnh_state_scan_args* a, const Plan& q, hipStream_t st) {
     p.channels = a->channels;
     p.states = (int)a->states;
     p.softplus = a->softplus;
-    p.x = in(a->x), p.x_bs = a->x_batch_stride, p.x_s = a->x_stride;
-    p.delta = in(a->delta), p.delta_bs = a->delta_batch_stride, p.delta_s = a->delta_stride;
-    p.z = in(a->z), p.z_bs = a->z_batch_stride, p.z_s = a->z_stride;
+    auto bytes = [](int64_t stride) { return (uint32_t)(stride * (int64_t)sizeof(T)); }; // checked by the caller
+    p.x = in(a->x), p.x_bs = a->x_batch_stride, p.x_s = bytes(a->x_stride);
+    p.delta = in(a->delta), p.delta_bs = a->delta_batch_stride, p.delta_s = bytes(a->delta_stride);
+    p.z = in(a->z), p.z_bs = a->z_batch_stride, p.z_s = bytes(a->z_stride);
     p.A = in(a->A);
-    p.B = in(a->B), p.B_bs = a->B_batch_stride, p.B_s = a->B_stride;
-    p.C = in(a->C), p.C_bs = a->C_batch_stride, p.C_s = a->C_stride;
+    p.B = in(a->B), p.B_bs = a->B_batch_stride, p.B_s = bytes(a->B_stride);
+    p.C = in(a->C), p.C_bs = a->C_batch_stride, p.C_s = bytes(a->C_stride);
     p.skip = in(a->skip);
     p.delta_bias = in(a->delta_bias);
     p.state_in = in(a->state_in);
     p.state_out = static_cast<T*>(a->state_out);
     p.lengths = a->lengths;
-    p.y = static_cast<T*>(a->y), p.y_bs = a->y_batch_stride, p.y_s = a->y_stride;
+    p.y = static_cast<T*>(a->y), p.y_bs = a->y_batch_stride, p.y_s = bytes(a->y_stride);
     p.piece = q.piece;
     p.pieces = q.pieces;
     p.carry = static_cast<T*>(a->workspace);
@@ -523,7 +643,7 @@ int run(const cnh_state_scan_args* a, const Plan& q, hipStream_t st) {
     auto fits = [&](const void* ptr, int64_t outer, int64_t inner) {
         return aligned_to(ptr, 16) && (p.batch == 1 || outer % W == 0) && (p.length <= 1 || inner % W == 0);
     };
-    const bool wide = fits(p.B, p.B_bs, p.B_s) && fits(p.C, p.C_bs, p.C_s);
+    const bool wide = fits(p.B, p.B_bs, a->B_stride) && fits(p.C, p.C_bs, a->C_stride);
     if (q.npl == 4) {
         switch (q.lanes) {
         case 1: return launch_full<T, 4, 1>(p, wide, st);
@@ -535,9 +655,10 @@ int run(const cnh_state_scan_args* a, const Plan& q, hipStream_t st) {
     }
     if (q.npl == 8)
         return launch_full<T, 8, 1>(p, wide, st);
+    if (q.npl == 32)
+        return launch_full<T, 32, 1>(p, wide, st);
     switch (q.lanes) {
     case 1: return launch_full<T, 16, 1>(p, wide, st);
-    case 2: return launch_full<T, 16, 2>(p, wide, st);
     case 4: return launch_full<T, 16, 4>(p, wide, st);
     case 8: return launch_full<T, 16, 8>(p, wide, st);
     default: return launch_full<T, 16, 16>(p, wide, st);
@@ -604,6 +725,10 @@ extern "C" int cnh_state_scan(const cnh_state_scan_args* a, cnh_stream s) {
             return rc;
     if (int rc = check_extent(len, 4, call))
         return rc;
+    if (a->length > 1)
+        for (int64_t stride : {a->x_stride, a->delta_stride, a->z ? a->z_stride : 0, a->B_stride, a->C_stride, a->y_stride})
+            CNH_CHECK(stride < ((int64_t)1 << 31) / esz, -3, "%s: %lld elements between tokens; rows are less than 2 GiB apart",
+                      call, (long long)stride);
     CNH_CHECK(q.bytes == 0 || (a->workspace && a->workspace_bytes >= q.bytes), -2,
               "%s: a workspace of %lld bytes is needed, %lld given", call, (long long)q.bytes,
               (long long)(a->workspace ? a->workspace_bytes : 0));
