@@ -573,8 +573,11 @@ Plan plan_of(const cnh_state_scan_args* a) {
         q.piece = std::max<int64_t>(1, (a->batch + slices - 1) / slices);
         q.piece = std::max(q.piece, (a->batch + 65534) / 65535);
     } else {
-        if (w < 3 * kUnits / 2 && w > 0)
-            q.pieces = (int)std::max<int64_t>(1, std::min(4 * kUnits / w, L / 16));
+        // Measured with 300 tokens of 2048 fp32 channels, 16 states: 16 sequences (512 wavefronts) 120 us
+        // uncut, 95 us in 8 pieces; 24 sequences (768) 129 us uncut, 134 us in 3. With 256 channels of
+        // 2 sequences: 64 tokens 20 us uncut, 22 us in 4 pieces; 128 tokens 29 and 22 us.
+        if (w <= kUnits / 2 && w > 0 && L >= 96)
+            q.pieces = (int)std::min(4 * kUnits / w, L / 16);
         q.piece = (L + q.pieces - 1) / q.pieces;
         q.pieces = (int)((L + q.piece - 1) / q.piece);
     }
