@@ -18,6 +18,9 @@
 // A word 32 below the maximum (e^-32 < 2^-46) has no mass and is never drawn. Exponentials and depths are
 // 64-bit whatever the logits' type: the drawn word changes where a running sum passes the random number.
 //
+// Few rows whose every word has to be weighed are cut into slices: a pass for the slices' maxima, one that
+// adds their weights up bin by bin in the workspace, and the row's own workgroup goes on from there.
+//
 // Bound by memory for many rows (one workgroup per row, the passes behind the first come from the
 // caches) and by the length of one row's passes for few.
 #include "sequence.h"
@@ -44,6 +47,13 @@ struct SampleParams {
     const double *top_ps, *min_ps;
     int32_t* out;
     double mass_scale; // mass of weight 1
+    // Few rows: each is cut into slices that other workgroups weigh first. One entry per slice, per bin
+    // or per row, rows one behind the other.
+    int slices;
+    int64_t slice; // words, a multiple of what a 16-byte access takes
+    T* tops;
+    unsigned long long *masses, *above;
+    uint32_t* counts;
 };
 
 template <typename T>
@@ -75,6 +85,73 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 }
 __device__ __forceinline__ double value_of(uint64_t k) {
     return __longlong_as_double((long long)(k >> 63 ? k & ~(1ull << 63) : ~k));
+}
+
+// Lane exchange by the vector unit's row operations: no LDS round trip, and few bytes of code. A row's
+// phases run once each, so what they cost besides memory is mostly the fetching of their instructions.
+template <int CTRL, int ROWS, typename V>
+__device__ __forceinline__ V moved(V v) { // lanes without a source, and rows not in ROWS, get 0
+    if constexpr (sizeof(V) == 4) {
+        int i;
+        __builtin_memcpy(&i, &v, 4);
+        i = __builtin_amdgcn_update_dpp(0, i, CTRL, ROWS, 0xf, ROWS == 0xf);
+        __builtin_memcpy(&v, &i, 4);
+    } else {
+        int i[2];
+        __builtin_memcpy(i, &v, 8);
+        i[0] = __builtin_amdgcn_update_dpp(0, i[0], CTRL, ROWS, 0xf, ROWS == 0xf);
+        i[1] = __builtin_amdgcn_update_dpp(0, i[1], CTRL, ROWS, 0xf, ROWS == 0xf);
+        __builtin_memcpy(&v, i, 8);
+    }
+    return v;
+}
+template <typename V>
+__device__ __forceinline__ V of_lane(V v, int lane) { // lane: the same for the wavefront
+    if constexpr (sizeof(V) == 4) {
+        int i;
+        __builtin_memcpy(&i, &v, 4);
+        i = __builtin_amdgcn_readlane(i, lane);
+        __builtin_memcpy(&v, &i, 4);
+    } else {
+        int i[2];
+        __builtin_memcpy(i, &v, 8);
+        i[0] = __builtin_amdgcn_readlane(i[0], lane);
+        i[1] = __builtin_amdgcn_readlane(i[1], lane);
+        __builtin_memcpy(&v, i, 8);
+    }
+    return v;
+}
+// Sums over the lanes of a row of 16 up to this one; of a wavefront.
+template <typename V>
+__device__ __forceinline__ V row_sums(V v) {
+    v += moved<0x111, 0xf>(v); // row_shr 1, 2, 4, 8
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    return v;
+}
+template <typename V>
+__device__ __forceinline__ V wave_sums(V v) {
+    v = row_sums(v);
+    v += moved<0x142, 0xa>(v); // row_bcast 15 to the odd rows
+    v += moved<0x143, 0xc>(v); // row_bcast 31 to the upper two
+    return v;
+}
+// The largest value of a row of 16, in all its lanes; of a wavefront.
+template <typename V>
+__device__ __forceinline__ V larger(V a, V b) { return b > a ? b : a; }
+template <typename V>
+__device__ __forceinline__ V row_max(V v) {
+    v = larger(v, moved<0xB1, 0xf>(v));  // quad_perm [1,0,3,2]
+    v = larger(v, moved<0x4E, 0xf>(v));  // quad_perm [2,3,0,1]
+    v = larger(v, moved<0x141, 0xf>(v)); // row_half_mirror
+    v = larger(v, moved<0x140, 0xf>(v)); // row_mirror
+    return v;
+}
+template <typename V>
+__device__ __forceinline__ V wave_max(V v) {
+    v = row_max(v);
+    return larger(larger(of_lane(v, 0), of_lane(v, 16)), larger(of_lane(v, 32), of_lane(v, 48)));
 }
 
 template <typename T>
@@ -173,10 +250,16 @@ struct Row {
         e = fma(e, r, 1.0);
         return e * sh.level[bin];
     }
+    bool weighed; // by weight_at(), which the list then goes by as well; the levels are there
     __device__ __forceinline__ double weight(T l) const {
         double r;
-        const int bin = bin_at(depth(l), &r);
-        return bin < kBins ? weight_at(bin, r) : 0.0;
+        const double d = depth(l);
+        const int bin = bin_at(d, &r);
+        return weighed ? weight_at(bin, r) : bin < kBins ? exp(-d) : 0.0;
+    }
+    __device__ __forceinline__ void fill_levels() const {
+        for (int b = tid; b <= kBins; b += kThreads)
+            sh.level[b] = b < kBins ? exp(-b / kBinsPerUnit) : 0.0;
     }
     // w * scale below 2^52: adding 2^52 leaves the rounded integer in the low bits
     __device__ __forceinline__ unsigned long long mass_of(double w) const {
@@ -235,20 +318,14 @@ struct Row {
     // Sum of v over the lanes up to this one, of the whole workgroup.
     template <typename V>
     __device__ __forceinline__ V running_sum(V v, V* waves) const {
-        const int lane = tid & 63;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const V up = __shfl_up(v, o, 64);
-            if (lane >= o)
-                v += up;
-        }
-        if (lane == 63)
-            waves[tid >> 6] = v;
+        static_assert(kWaves == 16, "a row of lanes");
+        v = wave_sums(v);
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        if ((tid & 63) == 63)
+            waves[wave] = v;
         __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kWaves - 1; ++w)
-            v += w < tid >> 6 ? waves[w] : V(0);
-        return v;
+        const V upto = row_sums(waves[tid & 15]);
+        return wave ? v + of_lane(upto, wave - 1) : v;
     }
     // Turns a histogram into running sums (each bin's own included). Two bins a lane.
     __device__ __forceinline__ void running_sums(uint32_t* count, unsigned long long* mass) {
@@ -268,16 +345,17 @@ struct Row {
         if (tid == 0)
             sh.found = kBins;
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int b = 2 * tid + j;
-            if (done(count[b], mass[b]) && (b == 0 || !done(count[b - 1], mass[b - 1])))
-                sh.found = b; // one lane at most
-        }
+        if (first_lane(done(count[2 * tid + 1], mass[2 * tid + 1])))
+            atomicMin(&sh.found, done(count[2 * tid], mass[2 * tid]) ? 2 * tid : 2 * tid + 1);
         __syncthreads();
         const uint32_t b = sh.found;
         __syncthreads();
         return b;
+    }
+    // Is this the first lane of its wavefront with `yes`?
+    __device__ __forceinline__ bool first_lane(bool yes) const {
+        const unsigned long long all = __ballot(yes);
+        return yes && (all & ((1ull << (tid & 63)) - 1)) == 0;
     }
 
     __device__ __forceinline__ void clear(uint32_t* count, unsigned long long* mass) {
@@ -377,7 +455,7 @@ struct Row {
         if (tid == 0)
             sh.found = n;
         __syncthreads();
-        if (tid < n && done(tid) && (tid == 0 || !done(tid - 1)))
+        if (first_lane(tid < n && done(tid)))
             atomicMin(&sh.found, (uint32_t)tid);
         __syncthreads();
         const uint32_t i = sh.found;
@@ -501,131 +579,226 @@ struct Row {
     }
 };
 
+// What a row asks for, with entries outside their range held to it.
+struct Settings {
+    double temperature, top_p, min_p;
+    int64_t top_k;
+    bool greedy, weigh; // the largest logit; every word's weight is needed
+    template <typename T>
+    __device__ __forceinline__ Settings(const SampleParams<T>& p, int64_t row) {
+        temperature = p.temperatures ? p.temperatures[row] : p.temperature;
+        top_p = p.top_ps ? p.top_ps[row] : p.top_p;
+        min_p = p.min_ps ? p.min_ps[row] : p.min_p;
+        min_p = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
+        top_k = p.top_ks ? p.top_ks[row] : p.top_k;
+        greedy = !(temperature > 0.0 && top_k != 1 && !(top_p <= 0.0));
+        // a small top-k is cut by the lanes' maxima
+        weigh = !(top_k > 0 && top_k <= kThreads / 2);
+    }
+};
+
+// Adds the weights of the row's words to the bins of sh.mass, their numbers to those of sh.count when
+// `counted`; returns this lane's part of the mass of those that weigh min_p or more. No branches, so that a
+// pack's words go through the long chains side by side: what is out of reach adds nothing to the bin
+// beyond the last.
+template <typename T>
+__device__ __forceinline__ unsigned long long weigh_words(const Row<T>& r, Shared<T>& sh, double min_p, bool counted) {
+    unsigned long long own = 0;
+    r.sweep([&](const auto& q, uint32_t) {
+        constexpr int N = (int)(sizeof(q.v) / sizeof(T));
+        int b[N];
+        double w[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            double rest;
+            b[j] = r.bin_at(r.depth(q.v[j]), &rest);
+            w[j] = r.weight_at(b[j], rest);
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            atomicAdd(&sh.mass[b[j]], r.mass_of(w[j]));
+        if (min_p > 0.0)
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                own += b[j] < kBins && w[j] >= min_p ? r.mass_of(w[j]) : 0;
+        if (counted)
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                atomicAdd(&sh.count[b[j]], 1u);
+    });
+    return own;
+}
+
+// The largest logit that the lanes hold, in all of them.
+template <typename T>
+__device__ __forceinline__ T group_max(T v, Shared<T>& sh) {
+    v = wave_max(v);
+    if ((threadIdx.x & 63) == 0)
+        sh.wave_top[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return row_max(sh.wave_top[threadIdx.x & 15]);
+}
+template <typename T>
+__device__ __forceinline__ T own_max(const Row<T>& r) {
+    T top = -std::numeric_limits<T>::infinity();
+    r.sweep([&](const auto& q, uint32_t) {
+#pragma unroll
+        for (int j = 0; j < (int)(sizeof(q.v) / sizeof(T)); ++j)
+            top = q.v[j] > top ? q.v[j] : top; // NaN: never
+    });
+    return top;
+}
+
+// A slice of a row: its largest logit; and zeros where the slices' weights will be added up.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void slice_top_kernel(SampleParams<T> p) {
+    __shared__ Shared<T> sh;
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.y, first = blockIdx.x * p.slice;
+    const Row<T> r{sh, p.logits + row * p.stride + first, std::min(p.slice, p.vocab - first), 0.0, 0.0, 0.0, tid, false};
+    const T top = group_max(own_max(r), sh);
+    if (tid == 0)
+        p.tops[row * p.slices + blockIdx.x] = top;
+    for (int b = blockIdx.x * kThreads + tid; b < kBins; b += p.slices * kThreads) {
+        p.masses[row * kBins + b] = 0;
+        p.counts[row * kBins + b] = 0;
+    }
+    if (blockIdx.x == 0 && tid == 0)
+        p.above[row] = 0;
+}
+
+// A slice of a row: its words weighed, and what its bins hold added to the row's.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void slice_weigh_kernel(SampleParams<T> p) {
+    __shared__ Shared<T> sh;
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.y, first = blockIdx.x * p.slice;
+    const Settings q(p, row);
+    T top = -std::numeric_limits<T>::infinity();
+    for (int i = 0; i < p.slices; ++i)
+        top = std::max(top, p.tops[row * p.slices + i]);
+    if (q.greedy || !q.weigh || !(fabs((double)top) <= (double)std::numeric_limits<T>::max()))
+        return; // the same for the whole workgroup
+    Row<T> r{sh, p.logits + row * p.stride + first, std::min(p.slice, p.vocab - first), 0.0, 0.0, p.mass_scale, tid, true};
+    r.fill_levels();
+    r.set(top, q.temperature);
+    r.clear(sh.count, sh.mass); // and a barrier behind the levels
+    unsigned long long own = weigh_words(r, sh, q.min_p, q.top_k > 0);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int b = 2 * tid + j;
+        if (sh.mass[b])
+            atomicAdd(&p.masses[row * kBins + b], sh.mass[b]);
+        if (sh.count[b])
+            atomicAdd(&p.counts[row * kBins + b], sh.count[b]);
+    }
+    own = wave_sums(own);
+    if ((tid & 63) == 63 && own)
+        atomicAdd(&p.above[row], own);
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams<T> p) {
     typedef typename KeyOf<T>::type Key;
     __shared__ Shared<T> sh;
     const int tid = threadIdx.x;
-    for (int b = tid; b <= kBins; b += kThreads)
-        sh.level[b] = b < kBins ? exp(-b / kBinsPerUnit) : 0.0;
+    bool levels = false; // filled for the first row that needs them
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        Row<T> r{sh, p.logits + row * p.stride, p.vocab, 0.0, 0.0, p.mass_scale, tid};
-        const double temperature = p.temperatures ? p.temperatures[row] : p.temperature;
-        const double top_p = p.top_ps ? p.top_ps[row] : p.top_p;
-        double min_p = p.min_ps ? p.min_ps[row] : p.min_p;
-        min_p = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
-        const int64_t top_k = p.top_ks ? p.top_ks[row] : p.top_k;
+        Row<T> r{sh, p.logits + row * p.stride, p.vocab, 0.0, 0.0, p.mass_scale, tid, false};
+        const Settings q(p, row);
+        const double top_p = q.top_p, min_p = q.min_p;
+        const int64_t top_k = q.top_k;
         const double u0 = p.u[row], u = u0 > 0.0 ? fmin(u0, 1.0) : 0.0;
+        bool weigh = q.weigh;
+        bool weighed = p.slices > 1 && weigh; // by the slices
 
         // the largest logit; each lane keeps its own
         const T none = -std::numeric_limits<T>::infinity();
         T own_top = none;
-        r.sweep([&](const auto& q, uint32_t) {
-#pragma unroll
-            for (int j = 0; j < (int)(sizeof(q.v) / sizeof(T)); ++j)
-                own_top = q.v[j] > own_top ? q.v[j] : own_top; // NaN: never
-        });
-        T top = own_top;
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) {
-            const T other = __shfl_xor(top, o, 64);
-            top = other > top ? other : top;
-        }
-        if ((tid & 63) == 0)
-            sh.wave_top[tid >> 6] = top;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w)
-            top = sh.wave_top[w] > top ? sh.wave_top[w] : top;
+        if (weighed)
+            own_top = tid < p.slices ? p.tops[row * p.slices + tid] : none;
+        else
+            own_top = own_max(r);
+        const T top = group_max(own_top, sh);
 
         int32_t drawn = -1;        // every word is masked (or no number)
         T value = top;             // where a place among words of one value decides: the value, and which of
         uint32_t nth = 0;          // them, counted from 1
-        const bool greedy = !(temperature > 0.0 && top_k != 1 && !(top_p <= 0.0));
-        if (top > none && greedy) {
+        if (top > none && q.greedy) {
             nth = 1;
         } else if (top > std::numeric_limits<T>::max()) {
             nth = r.among_infinite(top, top_k, top_p, u);
         } else if (top > none) {
-            r.set(top, temperature);
+            r.set(top, q.temperature);
             auto target_of = [&](unsigned long long kept) {
                 return min((unsigned long long)(u * (double)kept), kept - 1);
             };
-            // A small top-k is cut by the lanes' maxima; other rows weigh every word.
-            bool weigh = !(top_k > 0 && top_k <= kThreads / 2);
+            const bool short_row = p.vocab <= kList; // a list takes all of it: no bins, no cut in front
+            if (short_row)
+                weigh = weighed = false;
             for (bool again = true; again;) {
                 again = false;
-                r.clear(sh.count, sh.mass);
-                unsigned long long own = 0;
-                if (weigh) {
-                    // no branches, so that a pack's words go through the long chains side by side: what is
-                    // out of reach adds nothing to the bin beyond the last
-                    r.sweep([&](const auto& q, uint32_t) {
-                        constexpr int N = (int)(sizeof(q.v) / sizeof(T));
-                        int b[N];
-                        double w[N];
-#pragma unroll
-                        for (int j = 0; j < N; ++j) {
-                            double rest;
-                            b[j] = r.bin_at(r.depth(q.v[j]), &rest);
-                            w[j] = r.weight_at(b[j], rest);
-                        }
-#pragma unroll
-                        for (int j = 0; j < N; ++j)
-                            atomicAdd(&sh.mass[b[j]], r.mass_of(w[j]));
-                        if (min_p > 0.0)
-#pragma unroll
-                            for (int j = 0; j < N; ++j)
-                                own += b[j] < kBins && w[j] >= min_p ? r.mass_of(w[j]) : 0;
-                        if (top_k > 0)
-#pragma unroll
-                            for (int j = 0; j < N; ++j)
-                                atomicAdd(&sh.count[b[j]], 1u);
-                    });
-                } else if (own_top > none) {
-                    atomicAdd(&sh.count[r.bin_of(own_top)], 1u);
-                }
-                __syncthreads();
-                if (weigh && !(top_k > 0)) {
-                    // nobody counts: a bin's words weigh its level times e^(-1/128) or more, which
-                    // tells how many they are nearly enough to decide whether a list takes them
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int b = 2 * tid + j;
-                        const double each = fmax(sh.level[b] * 0.992 * p.mass_scale, 1.0);
-                        sh.count[b] = (uint32_t)fmin(ceil((double)sh.mass[b] / each), (double)p.vocab);
-                    }
-                }
-                r.running_sums(sh.count, sh.mass);
-                const uint32_t words = sh.count[kBins - 1];
-                const unsigned long long total = sh.mass[kBins - 1];
-                auto count_of = [&](uint32_t b0, uint32_t b1) { return sh.count[b1] - (b0 ? sh.count[b0 - 1] : 0); };
-                Until until{Until::COUNT, (uint32_t)max(top_k, (int64_t)0), top_p * (double)total, 0};
+                unsigned long long own = 0, total = 0;
                 uint32_t by_k = kBins, by_p = kBins, by_min_p = kBins;
-                if (top_k > 0 && top_k <= (int64_t)words)
-                    by_k = r.first_bin(sh.count, sh.mass, until);
-                until.kind = Until::REACHED;
-                if (weigh && top_p < 1.0)
-                    by_p = r.first_bin(sh.count, sh.mass, until);
+                Until until{Until::REACHED, (uint32_t)max(top_k, (int64_t)0), 0.0, 0};
+                r.weighed = weigh;
+                if (weigh && !levels) {
+                    r.fill_levels();
+                    levels = true;
+                }
+                if (!short_row) {
+                    r.clear(sh.count, sh.mass);
+                    if (weighed) {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const int b = 2 * tid + j;
+                            sh.mass[b] = p.masses[row * kBins + b];
+                            sh.count[b] = p.counts[row * kBins + b];
+                        }
+                        own = tid == 0 ? p.above[row] : 0;
+                    } else if (weigh) {
+                        own = weigh_words(r, sh, min_p, top_k > 0);
+                    } else if (own_top > none) {
+                        atomicAdd(&sh.count[r.bin_of(own_top)], 1u);
+                    }
+                    __syncthreads();
+                    if (weigh && !(top_k > 0)) {
+                        // nobody counts: a bin's words weigh its level times e^(-1/128) or more, which
+                        // tells how many they are nearly enough to decide whether a list takes them
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const int b = 2 * tid + j;
+                            const double each = fmax(sh.level[b] * 0.992 * p.mass_scale, 1.0);
+                            sh.count[b] = (uint32_t)fmin(ceil((double)sh.mass[b] / each), (double)p.vocab);
+                        }
+                    }
+                    r.running_sums(sh.count, sh.mass);
+                    total = sh.mass[kBins - 1];
+                    until.reached = top_p * (double)total;
+                    if (top_k > 0 && top_k <= (int64_t)sh.count[kBins - 1]) {
+                        until.kind = Until::COUNT;
+                        by_k = r.first_bin(sh.count, sh.mass, until);
+                        until.kind = Until::REACHED;
+                    }
+                    if (weigh && top_p < 1.0)
+                        by_p = r.first_bin(sh.count, sh.mass, until);
+                }
+                auto count_of = [&](uint32_t b0, uint32_t b1) { return sh.count[b1] - (b0 ? sh.count[b0 - 1] : 0); };
                 if (min_p > 0.0)
                     by_min_p = (uint32_t)fmin(-log(min_p) * kBinsPerUnit + 1.0, (double)kBins); // one to spare
                 uint32_t last = min(min(by_k, by_p), by_min_p); // last bin of a list of all that is kept
                 // p of what top-k leaves needs all of that in the list
-                if (top_p < 1.0 && top_k > 0 && (!weigh || by_k != kBins))
+                if (top_p < 1.0 && (!weigh || (top_k > 0 && by_k != kBins)))
                     last = by_k;
                 last = min(last, (uint32_t)kBins - 1);
                 if (weigh && min_p > 0.0) {
                     // mass of the words that min-p keeps: the sum of `own` over the workgroup
-#pragma unroll
-                    for (int o = 32; o >= 1; o >>= 1)
-                        own += __shfl_xor(own, o, 64);
-                    if ((tid & 63) == 0)
+                    own = wave_sums(own);
+                    if ((tid & 63) == 63)
                         sh.wave_mass[tid >> 6] = own;
                     __syncthreads();
-                    own = 0;
-#pragma unroll
-                    for (int w = 0; w < kWaves; ++w)
-                        own += sh.wave_mass[w];
+                    own = of_lane(row_sums(sh.wave_mass[tid & 15]), 15);
                     __syncthreads();
                 }
 
@@ -770,8 +943,28 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams<T> p) {
     }
 }
 
+// Slices per row and the workspace for what they leave: host arithmetic on the sizes and on what the
+// settings can ask for.
+struct Plan {
+    int slices;
+    int64_t slice, bytes;
+};
+Plan plan_of(const cnh_sample_tokens_args* a) {
+    Plan q{1, a->vocab, 0};
+    const bool weighs = (a->top_ks || a->top_k == 0 || a->top_k > kThreads / 2) && (a->temperatures || a->temperature > 0.0);
+    // One workgroup reads and weighs a word a lane at a time: a slice of 8192 words takes it 3 us, about what
+    // the two more launches cost.
+    if (weighs && a->rows > 0)
+        q.slices = (int)std::max<int64_t>(1, std::min<int64_t>({16, 256 / a->rows, a->vocab / 8192}));
+    if (q.slices > 1) {
+        q.slice = ((a->vocab + q.slices - 1) / q.slices + 3) / 4 * 4;
+        q.bytes = a->rows * (kBins * 12 + 8 + q.slices * (int64_t)dtype_size(a->dtype));
+    }
+    return q;
+}
+
 template <typename T>
-int run(const cnh_sample_tokens_args* a, hipStream_t st) {
+int run(const cnh_sample_tokens_args* a, const Plan& q, hipStream_t st) {
     SampleParams<T> p;
     p.rows = a->rows;
     p.vocab = a->vocab;
@@ -791,6 +984,17 @@ int run(const cnh_sample_tokens_args* a, hipStream_t st) {
     while (((int64_t)1 << bits) < a->vocab)
         ++bits;
     p.mass_scale = (double)((uint64_t)1 << std::min(45, 62 - bits));
+    p.slices = q.slices;
+    p.slice = q.slice;
+    p.masses = static_cast<unsigned long long*>(a->workspace);
+    p.above = p.masses + p.rows * kBins;
+    p.tops = reinterpret_cast<T*>(p.above + p.rows);
+    p.counts = reinterpret_cast<uint32_t*>(p.tops + p.rows * p.slices);
+    if (p.slices > 1) {
+        const dim3 grid(p.slices, (unsigned)p.rows);
+        slice_top_kernel<T><<<grid, kThreads, 0, st>>>(p);
+        slice_weigh_kernel<T><<<grid, kThreads, 0, st>>>(p);
+    }
     sample_kernel<T><<<(unsigned)std::min<int64_t>(p.rows, 1 << 20), kThreads, 0, st>>>(p);
     CNH_HIP(hipGetLastError());
     return 0;
@@ -809,7 +1013,9 @@ int check(const cnh_sample_tokens_args* a, const char* call) {
 } // namespace
 
 extern "C" int64_t cnh_sample_tokens_workspace(const cnh_sample_tokens_args* a) {
-    return check(a, "cnh_sample_tokens_workspace");
+    if (int rc = check(a, "cnh_sample_tokens_workspace"))
+        return rc;
+    return plan_of(a).bytes;
 }
 
 extern "C" int cnh_sample_tokens(const cnh_sample_tokens_args* a, cnh_stream s) {
@@ -842,10 +1048,18 @@ extern "C" int cnh_sample_tokens(const cnh_sample_tokens_args* a, cnh_stream s) 
         CNH_CHECK(!overlap(out, e), -2, "%s: out overlaps %s", call, e.what);
     }
     CNH_CHECK(!overlap(out, logits) && !overlap(out, ks), -2, "%s: out overlaps logits or top_ks", call);
+    const Plan q = plan_of(a);
+    const Extent ws{"workspace", a->workspace, q.bytes};
+    CNH_CHECK(q.bytes == 0 || (a->workspace && a->workspace_bytes >= q.bytes), -2,
+              "%s: a workspace of %lld bytes is needed, %lld given", call, (long long)q.bytes,
+              (long long)(a->workspace ? a->workspace_bytes : 0));
+    CNH_CHECK(q.bytes == 0 || aligned_to(a->workspace, 16), -2, "%s: the workspace is not aligned to 16 bytes", call);
+    for (const Extent* e : {&out, &logits, &ks, &doubles[0], &doubles[1], &doubles[2], &doubles[3]})
+        CNH_CHECK(!overlap(ws, *e), -2, "%s: the workspace overlaps %s", call, e->what);
     if (int rc = ensure_init())
         return rc;
     DeviceScope dev;
     if (int rc = dev.enter())
         return rc;
-    return a->dtype == CNH_F32 ? run<float>(a, as_stream(s)) : run<double>(a, as_stream(s));
+    return a->dtype == CNH_F32 ? run<float>(a, q, as_stream(s)) : run<double>(a, q, as_stream(s));
 }

@@ -387,3 +387,33 @@ def test_sample_follows_the_weights(dev):
     # n evenly spaced numbers meet an interval of length l between n l - 1 and n l + 1 times
     assert (np.abs(np.bincount(got, minlength=V) - n * w / w.sum()) <= 1 + 1e-6).all()
     dev.free_all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_few_long_rows(dev, dtype):
+    """Rows long enough to be weighed in slices, all kinds of them in one call: the slices of rows that are
+    not weighed, masked or infinite, and crowds that lie in several slices."""
+    rng = np.random.default_rng(12)
+    V = 40003
+    x = (2 * rng.standard_normal((12, V))).astype(dtype)
+    x[3] = -np.inf
+    x[4, 5:V:7] = np.inf
+    x[5] = np.finfo(dtype).min
+    x[6] = 1.5
+    x[7, : V // 2] = -np.inf                              # nothing in the first slices
+    x[8] = np.nan
+    x[9, 1:] = -np.inf                                    # a single word
+    x[10] = rng.integers(0, 2, V)
+    u = rng.random(12)
+    t = np.array([1.0, 0.8, 0.0, 1, 1, 1, 1, 1.2, 1, 1, 0.9, 2.0])
+    k = np.array([0, 3, 7, 0, 9000, 0, 30000, 0, 0, 0, 25000, 5000])
+    p = np.array([0.9, 0.9, 1, 1, 0.4, 0.7, 0.6, 1.0, 1, 0.3, 0.99, 0.8])
+    m = np.array([0, 0, 0, 0, 0.1, 0.5, 0, 0.01, 0, 0.2, 0, 0])
+    got = sample_call(dev, x, u, t, k, p, m)
+    check_rows(got, x, u, t, k, p, m)
+    assert got[3] == got[8] == -1 and got[9] == 0 and got[4] % 7 == 5
+    again = sample_call(dev, x, u, t, k, p, m)
+    assert np.array_equal(got, again)
+    one = np.concatenate([sample_call(dev, x[r:r + 1], u[r:r + 1], t[r], int(k[r]), p[r], m[r]) for r in range(12)])
+    assert np.array_equal(got, one)                       # the same word however many rows and slices there are
+    dev.free_all()

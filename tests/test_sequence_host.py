@@ -114,6 +114,11 @@ NAN = float("nan")
     (scan, dict(length=4096, x_batch_stride=1 << 15, delta_batch_stride=1 << 15, z_batch_stride=1 << 15,
                 B_batch_stride=1 << 16, C_batch_stride=1 << 16, y_batch_stride=1 << 15), -2, "workspace of"),
     (sample, dict(dtype=L.I32), -2, "element type"),
+    (sample, dict(vocab=1 << 17, stride=1 << 17, u=10 * BIG, out=11 * BIG), -2, "workspace of"),
+    (sample, dict(vocab=1 << 17, stride=1 << 17, u=10 * BIG, out=11 * BIG, workspace=12 * BIG, workspace_bytes=9), -2,
+     "workspace of"),
+    (sample, dict(vocab=1 << 17, stride=1 << 17, u=10 * BIG, out=11 * BIG, workspace=10 * BIG, workspace_bytes=BIG), -2,
+     "workspace overlaps u"),
     (sample, dict(vocab=0), -3, "words"),
     (sample, dict(vocab=(1 << 22) + 1), -3, "words"),
     (sample, dict(rows=-1), -3, "rows"),
@@ -158,4 +163,10 @@ def test_workspaces():
     assert one > 0 and one % (17 * 2048 * 4) == 0
     assert need(batch=1, channels=2048, length=8192, dtype=L.F64) == 2 * one
     assert need(states=500) == -3
-    assert L.lib.cnh_sample_tokens_workspace(C.byref(sample())) >= 0
+    words = lambda **kw: L.lib.cnh_sample_tokens_workspace(C.byref(sample(**kw)))  # noqa: E731
+    assert words() == 0
+    # a histogram of 2048 masses and counts, the mass above min-p and the slices' maxima for each row
+    assert words(rows=2, vocab=131072, stride=131072) == 2 * (2048 * 12 + 8 + 16 * 4)
+    assert words(rows=2, vocab=131072, top_k=50) == 0 and words(rows=2, vocab=131072, temperature=0.0) == 0
+    assert words(rows=2, vocab=131072, top_k=50, top_ks=BIG * 9) > 0
+    assert words(rows=200, vocab=131072) == 0 and words(vocab=-1) == -3
