@@ -33,10 +33,11 @@ struct NormParams {
 
 template <typename T>
 __device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1)
-        v += __shfl_xor(v, o, 64);
-    return v;
+    v += moved<0xB1, 0xf>(v);  // quad_perm [1,0,3,2]
+    v += moved<0x4E, 0xf>(v);  // quad_perm [2,3,0,1]
+    v += moved<0x141, 0xf>(v); // row_half_mirror
+    v += moved<0x140, 0xf>(v); // row_mirror
+    return (of_lane(v, 0) + of_lane(v, 16)) + (of_lane(v, 32) + of_lane(v, 48));
 }
 
 // Sum over the WAVES wavefronts of a row, the same value in every lane.

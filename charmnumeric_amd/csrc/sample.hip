@@ -87,40 +87,9 @@ __device__ __forceinline__ double value_of(uint64_t k) {
     return __longlong_as_double((long long)(k >> 63 ? k & ~(1ull << 63) : ~k));
 }
 
-// Lane exchange by the vector unit's row operations: no LDS round trip, and few bytes of code. A row's
-// phases run once each, so what they cost besides memory is mostly the fetching of their instructions.
-template <int CTRL, int ROWS, typename V>
-__device__ __forceinline__ V moved(V v) { // lanes without a source, and rows not in ROWS, get 0
-    if constexpr (sizeof(V) == 4) {
-        int i;
-        __builtin_memcpy(&i, &v, 4);
-        i = __builtin_amdgcn_update_dpp(0, i, CTRL, ROWS, 0xf, ROWS == 0xf);
-        __builtin_memcpy(&v, &i, 4);
-    } else {
-        int i[2];
-        __builtin_memcpy(i, &v, 8);
-        i[0] = __builtin_amdgcn_update_dpp(0, i[0], CTRL, ROWS, 0xf, ROWS == 0xf);
-        i[1] = __builtin_amdgcn_update_dpp(0, i[1], CTRL, ROWS, 0xf, ROWS == 0xf);
-        __builtin_memcpy(&v, i, 8);
-    }
-    return v;
-}
-template <typename V>
-__device__ __forceinline__ V of_lane(V v, int lane) { // lane: the same for the wavefront
-    if constexpr (sizeof(V) == 4) {
-        int i;
-        __builtin_memcpy(&i, &v, 4);
-        i = __builtin_amdgcn_readlane(i, lane);
-        __builtin_memcpy(&v, &i, 4);
-    } else {
-        int i[2];
-        __builtin_memcpy(i, &v, 8);
-        i[0] = __builtin_amdgcn_readlane(i[0], lane);
-        i[1] = __builtin_amdgcn_readlane(i[1], lane);
-        __builtin_memcpy(&v, i, 8);
-    }
-    return v;
-}
+// A row's phases run once each, so what they cost besides memory is mostly the fetching of their
+// instructions: sums and maxima over the lanes by row operations are few of them.
+
 // Sums over the lanes of a row of 16 up to this one; of a wavefront.
 template <typename V>
 __device__ __forceinline__ V row_sums(V v) {

@@ -68,28 +68,17 @@ __device__ __forceinline__ float softplus(float v) {
 }
 __device__ __forceinline__ double softplus(double v) { return v > 40.0 ? v : log1p(exp(v)); }
 
-// v of the lane that a row operation of the vector unit pairs this one with
-template <int CTRL>
-__device__ __forceinline__ float partner(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
-}
-template <int CTRL>
-__device__ __forceinline__ double partner(double v) {
-    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, true);
-    const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, true);
-    return __hiloint2double(hi, lo);
-}
 // Sum over S neighbouring lanes, in every one of them.
 template <int S, typename T>
 __device__ __forceinline__ T lanes_sum(T v) {
     if (S >= 2)
-        v += partner<0xB1>(v); // quad_perm [1,0,3,2]
+        v += moved<0xB1, 0xf>(v); // quad_perm [1,0,3,2]
     if (S >= 4)
-        v += partner<0x4E>(v); // quad_perm [2,3,0,1]
+        v += moved<0x4E, 0xf>(v); // quad_perm [2,3,0,1]
     if (S >= 8)
-        v += partner<0x141>(v); // row_half_mirror
+        v += moved<0x141, 0xf>(v); // row_half_mirror
     if (S >= 16)
-        v += partner<0x140>(v); // row_mirror
+        v += moved<0x140, 0xf>(v); // row_mirror
     return v;
 }
 
@@ -107,7 +96,7 @@ __device__ __forceinline__ T& at(T* row, uint32_t bytes) {
 // v of lane U of every G neighbouring ones (G 2 or 4), in all of them.
 template <int G, int U, typename T>
 __device__ __forceinline__ T from_lane(T v) {
-    return partner<G == 4 ? U * 0x55 : U ? 0xF5 : 0xA0>(v);
+    return moved<(G == 4 ? U * 0x55 : U ? 0xF5 : 0xA0), 0xf>(v);
 }
 
 // A row so many bytes further.

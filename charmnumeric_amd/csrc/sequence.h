@@ -132,6 +132,39 @@ __device__ __forceinline__ void store_pack(const Pack<T, VEC>& p, T* at) {
     }
 }
 
+// Lane exchange by the vector unit's row operations (rows of 16 lanes): no LDS round trip.
+template <int CTRL, int ROWS, typename V>
+__device__ __forceinline__ V moved(V v) { // lanes without a source, and rows not in ROWS, get 0
+    if constexpr (sizeof(V) == 4) {
+        int i;
+        __builtin_memcpy(&i, &v, 4);
+        i = __builtin_amdgcn_update_dpp(0, i, CTRL, ROWS, 0xf, ROWS == 0xf);
+        __builtin_memcpy(&v, &i, 4);
+    } else {
+        int i[2];
+        __builtin_memcpy(i, &v, 8);
+        i[0] = __builtin_amdgcn_update_dpp(0, i[0], CTRL, ROWS, 0xf, ROWS == 0xf);
+        i[1] = __builtin_amdgcn_update_dpp(0, i[1], CTRL, ROWS, 0xf, ROWS == 0xf);
+        __builtin_memcpy(&v, i, 8);
+    }
+    return v;
+}
+template <typename V>
+__device__ __forceinline__ V of_lane(V v, int lane) { // lane: the same for the wavefront
+    if constexpr (sizeof(V) == 4) {
+        int i;
+        __builtin_memcpy(&i, &v, 4);
+        i = __builtin_amdgcn_readlane(i, lane);
+        __builtin_memcpy(&v, &i, 4);
+    } else {
+        int i[2];
+        __builtin_memcpy(i, &v, 8);
+        i[0] = __builtin_amdgcn_readlane(i[0], lane);
+        i[1] = __builtin_amdgcn_readlane(i[1], lane);
+        __builtin_memcpy(&v, i, 8);
+    }
+    return v;
+}
 // Tokens of sequence b that count: lengths[b] held to [0, length], or all of them.
 __device__ __forceinline__ int64_t tokens_of(const int32_t* lengths, int64_t b, int64_t length) {
     if (!lengths)
