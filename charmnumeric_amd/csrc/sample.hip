@@ -38,6 +38,7 @@ constexpr double kDepth = 32.0, kBinsPerUnit = kBins / kDepth;
 template <typename T>
 struct SampleParams {
     int64_t rows, vocab, stride;
+    int64_t first_row; // of this launch
     const T* logits;
     const double* u;
     double temperature, top_p, min_p;
@@ -239,7 +240,7 @@ struct Row {
     // of a lane at once, and what is before the first and behind the last whole one as packs of one.
     template <typename F>
     __device__ __forceinline__ void sweep(F f) const {
-        constexpr int VEC = Wide<T>::n, AHEAD = 4;
+        constexpr int VEC = Wide<T>::n, AHEAD = 2;
         const uint32_t words = (uint32_t)vocab;
         const uint32_t head = min((uint32_t)((16 - ((uintptr_t)logits & 15)) & 15) / (uint32_t)sizeof(T), words);
         const uint32_t packs = (words - head) / VEC;
@@ -323,8 +324,7 @@ struct Row {
     }
     // Is this the first lane of its wavefront with `yes`?
     __device__ __forceinline__ bool first_lane(bool yes) const {
-        const unsigned long long all = __ballot(yes);
-        return yes && (all & ((1ull << (tid & 63)) - 1)) == 0;
+        return yes && __ffsll(__ballot(yes)) - 1 == (tid & 63);
     }
 
     __device__ __forceinline__ void clear(uint32_t* count, unsigned long long* mass) {
@@ -521,7 +521,7 @@ struct Row {
                 before += w < tid >> 6 ? sh.wave_count[w] : 0;
                 all += sh.wave_count[w];
             }
-            if (hit && before + (uint32_t)__popcll(ballot & ((1ull << (tid & 63)) - 1)) + 1 == nth)
+            if (hit && before + __builtin_amdgcn_mbcnt_hi((uint32_t)(ballot >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)ballot, 0)) + 1 == nth)
                 sh.found = (uint32_t)i;
             seen = all;
             __syncthreads();
@@ -672,244 +672,239 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams<T> p) {
     typedef typename KeyOf<T>::type Key;
     __shared__ Shared<T> sh;
     const int tid = threadIdx.x;
-    bool levels = false; // filled for the first row that needs them
-    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        Row<T> r{sh, p.logits + row * p.stride, p.vocab, 0.0, 0.0, p.mass_scale, tid, false};
-        const Settings q(p, row);
-        const double top_p = q.top_p, min_p = q.min_p;
-        const int64_t top_k = q.top_k;
-        const double u0 = p.u[row], u = u0 > 0.0 ? fmin(u0, 1.0) : 0.0;
-        bool weigh = q.weigh;
-        bool weighed = p.slices > 1 && weigh; // by the slices
+    const int64_t row = p.first_row + blockIdx.x;
+    Row<T> r{sh, p.logits + row * p.stride, p.vocab, 0.0, 0.0, p.mass_scale, tid, false};
+    const Settings q(p, row);
+    const double top_p = q.top_p, min_p = q.min_p;
+    const int64_t top_k = q.top_k;
+    const double u0 = p.u[row], u = u0 > 0.0 ? fmin(u0, 1.0) : 0.0;
+    bool weigh = q.weigh;
+    bool weighed = p.slices > 1 && weigh; // by the slices
 
-        // the largest logit; each lane keeps its own
-        const T none = -std::numeric_limits<T>::infinity();
-        T own_top = none;
-        if (weighed)
-            own_top = tid < p.slices ? p.tops[row * p.slices + tid] : none;
-        else
-            own_top = own_max(r);
-        const T top = group_max(own_top, sh);
+    // the largest logit; each lane keeps its own
+    const T none = -std::numeric_limits<T>::infinity();
+    T own_top = none;
+    if (weighed)
+        own_top = tid < p.slices ? p.tops[row * p.slices + tid] : none;
+    else
+        own_top = own_max(r);
+    const T top = group_max(own_top, sh);
 
-        int32_t drawn = -1;        // every word is masked (or no number)
-        T value = top;             // where a place among words of one value decides: the value, and which of
-        uint32_t nth = 0;          // them, counted from 1
-        if (top > none && q.greedy) {
-            nth = 1;
-        } else if (top > std::numeric_limits<T>::max()) {
-            nth = r.among_infinite(top, top_k, top_p, u);
-        } else if (top > none) {
-            r.set(top, q.temperature);
-            auto target_of = [&](unsigned long long kept) {
-                return min((unsigned long long)(u * (double)kept), kept - 1);
-            };
-            const bool short_row = p.vocab <= kList; // a list takes all of it: no bins, no cut in front
-            if (short_row)
-                weigh = weighed = false;
-            for (bool again = true; again;) {
-                again = false;
-                unsigned long long own = 0, total = 0;
-                uint32_t by_k = kBins, by_p = kBins, by_min_p = kBins;
-                Until until{Until::REACHED, (uint32_t)max(top_k, (int64_t)0), 0.0, 0};
-                r.weighed = weigh;
-                if (weigh && !levels) {
-                    r.fill_levels();
-                    levels = true;
-                }
-                if (!short_row) {
-                    r.clear(sh.count, sh.mass);
-                    if (weighed) {
+    int32_t drawn = -1;        // every word is masked (or no number)
+    T value = top;             // where a place among words of one value decides: the value, and which of
+    uint32_t nth = 0;          // them, counted from 1
+    if (top > none && q.greedy) {
+        nth = 1;
+    } else if (top > std::numeric_limits<T>::max()) {
+        nth = r.among_infinite(top, top_k, top_p, u);
+    } else if (top > none) {
+        r.set(top, q.temperature);
+        auto target_of = [&](unsigned long long kept) {
+            return min((unsigned long long)(u * (double)kept), kept - 1);
+        };
+        const bool short_row = p.vocab <= kList; // a list takes all of it: no bins, no cut in front
+        if (short_row)
+            weigh = weighed = false;
+        for (bool again = true; again;) {
+            again = false;
+            unsigned long long own = 0, total = 0;
+            uint32_t by_k = kBins, by_p = kBins, by_min_p = kBins;
+            Until until{Until::REACHED, (uint32_t)max(top_k, (int64_t)0), 0.0, 0};
+            r.weighed = weigh;
+            if (weigh)
+                r.fill_levels();
+            if (!short_row) {
+                r.clear(sh.count, sh.mass);
+                if (weighed) {
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const int b = 2 * tid + j;
-                            sh.mass[b] = p.masses[row * kBins + b];
-                            sh.count[b] = p.counts[row * kBins + b];
-                        }
-                        own = tid == 0 ? p.above[row] : 0;
-                    } else if (weigh) {
-                        own = weigh_words(r, sh, min_p, top_k > 0);
-                    } else if (own_top > none) {
-                        atomicAdd(&sh.count[r.bin_of(own_top)], 1u);
+                    for (int j = 0; j < 2; ++j) {
+                        const int b = 2 * tid + j;
+                        sh.mass[b] = p.masses[row * kBins + b];
+                        sh.count[b] = p.counts[row * kBins + b];
                     }
-                    __syncthreads();
-                    if (weigh && !(top_k > 0)) {
-                        // nobody counts: a bin's words weigh its level times e^(-1/128) or more, which
-                        // tells how many they are nearly enough to decide whether a list takes them
+                    own = tid == 0 ? p.above[row] : 0;
+                } else if (weigh) {
+                    own = weigh_words(r, sh, min_p, top_k > 0);
+                } else if (own_top > none) {
+                    atomicAdd(&sh.count[r.bin_of(own_top)], 1u);
+                }
+                __syncthreads();
+                if (weigh && !(top_k > 0)) {
+                    // nobody counts: a bin's words weigh its level times e^(-1/128) or more, which
+                    // tells how many they are nearly enough to decide whether a list takes them
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const int b = 2 * tid + j;
-                            const double each = fmax(sh.level[b] * 0.992 * p.mass_scale, 1.0);
-                            sh.count[b] = (uint32_t)fmin(ceil((double)sh.mass[b] / each), (double)p.vocab);
-                        }
+                    for (int j = 0; j < 2; ++j) {
+                        const int b = 2 * tid + j;
+                        const double each = fmax(sh.level[b] * 0.992 * p.mass_scale, 1.0);
+                        sh.count[b] = (uint32_t)fmin(ceil((double)sh.mass[b] / each), (double)p.vocab);
                     }
-                    r.running_sums(sh.count, sh.mass);
-                    total = sh.mass[kBins - 1];
-                    until.reached = top_p * (double)total;
-                    if (top_k > 0 && top_k <= (int64_t)sh.count[kBins - 1]) {
-                        until.kind = Until::COUNT;
-                        by_k = r.first_bin(sh.count, sh.mass, until);
-                        until.kind = Until::REACHED;
-                    }
-                    if (weigh && top_p < 1.0)
-                        by_p = r.first_bin(sh.count, sh.mass, until);
                 }
-                auto count_of = [&](uint32_t b0, uint32_t b1) { return sh.count[b1] - (b0 ? sh.count[b0 - 1] : 0); };
-                if (min_p > 0.0)
-                    by_min_p = (uint32_t)fmin(-log(min_p) * kBinsPerUnit + 1.0, (double)kBins); // one to spare
-                uint32_t last = min(min(by_k, by_p), by_min_p); // last bin of a list of all that is kept
-                // p of what top-k leaves needs all of that in the list
-                if (top_p < 1.0 && (!weigh || (top_k > 0 && by_k != kBins)))
-                    last = by_k;
-                last = min(last, (uint32_t)kBins - 1);
-                if (weigh && min_p > 0.0) {
-                    // mass of the words that min-p keeps: the sum of `own` over the workgroup
-                    own = wave_sums(own);
-                    if ((tid & 63) == 63)
-                        sh.wave_mass[tid >> 6] = own;
-                    __syncthreads();
-                    own = of_lane(row_sums(sh.wave_mass[tid & 15]), 15);
-                    __syncthreads();
+                r.running_sums(sh.count, sh.mass);
+                total = sh.mass[kBins - 1];
+                until.reached = top_p * (double)total;
+                if (top_k > 0 && top_k <= (int64_t)sh.count[kBins - 1]) {
+                    until.kind = Until::COUNT;
+                    by_k = r.first_bin(sh.count, sh.mass, until);
+                    until.kind = Until::REACHED;
                 }
+                if (weigh && top_p < 1.0)
+                    by_p = r.first_bin(sh.count, sh.mass, until);
+            }
+            auto count_of = [&](uint32_t b0, uint32_t b1) { return sh.count[b1] - (b0 ? sh.count[b0 - 1] : 0); };
+            if (min_p > 0.0)
+                by_min_p = (uint32_t)fmin(-log(min_p) * kBinsPerUnit + 1.0, (double)kBins); // one to spare
+            uint32_t last = min(min(by_k, by_p), by_min_p); // last bin of a list of all that is kept
+            // p of what top-k leaves needs all of that in the list
+            if (top_p < 1.0 && (!weigh || (top_k > 0 && by_k != kBins)))
+                last = by_k;
+            last = min(last, (uint32_t)kBins - 1);
+            if (weigh && min_p > 0.0) {
+                // mass of the words that min-p keeps: the sum of `own` over the workgroup
+                own = wave_sums(own);
+                if ((tid & 63) == 63)
+                    sh.wave_mass[tid >> 6] = own;
+                __syncthreads();
+                own = of_lane(row_sums(sh.wave_mass[tid & 15]), 15);
+                __syncthreads();
+            }
 
-                // ALL: everything kept in one list. Otherwise the cuts one by one: by COUNT what top-k
-                // leaves, by MASS what top-p does; DRAW the word. Where top-p's cut is known to a bin the
-                // draw is known to a few: BOTH gathers the words of both.
-                enum { ALL, BY_COUNT, BOTH, BY_MASS, DRAW } stage = ALL;
-                unsigned long long most = total; // mass kept, as far as it is cut
-                Range<Key> g;
-                g.keyed = false;
-                uint32_t base_count = 0;
-                unsigned long long base_mass = 0;
-                if (weigh && sh.count[last] > kList)
-                    stage = by_k != kBins ? BY_COUNT : BOTH;
-                for (bool more = true; more;) {
-                    uint32_t n = kList + 1;
-                    if (!g.keyed) {
-                        if (stage == ALL) {
-                            g.b0 = 0;
-                            g.b1 = g.b2 = last;
-                            n = 0; // tried whatever the counts say: they may be those of the lanes' maxima
-                        } else if (stage == BOTH) {
-                            until.kind = Until::REACHED;
-                            const uint32_t cut = top_p < 1.0 ? r.first_bin(sh.count, sh.mass, until) : kBins;
-                            if (min_p > 0.0)
-                                most = min(most, own);
-                            if (cut == kBins || (cut ? sh.mass[cut - 1] : 0) >= most) {
-                                stage = DRAW; // top-p takes nothing away
-                                continue;
-                            }
-                            base_mass = cut ? sh.mass[cut - 1] : 0;
-                            until.kind = Until::PASSED;
-                            until.passed = target_of(max(base_mass, 1ull));
-                            g.b0 = r.first_bin(sh.count, sh.mass, until);
-                            until.passed = target_of(min(most, sh.mass[cut]));
-                            g.b1 = r.first_bin(sh.count, sh.mass, until);
-                            g.b2 = cut;
-                            n = count_of(g.b0, g.b1) + count_of(cut, cut);
-                        } else {
-                            until.kind = stage == BY_COUNT ? Until::COUNT : stage == BY_MASS ? Until::REACHED : Until::PASSED;
-                            until.passed = target_of(most);
-                            g.b0 = g.b1 = g.b2 = r.first_bin(sh.count, sh.mass, until);
-                            base_count = g.b2 ? sh.count[g.b2 - 1] : 0;
-                            base_mass = g.b2 ? sh.mass[g.b2 - 1] : 0;
-                            n = count_of(g.b2, g.b2);
-                        }
-                    } else {
-                        n = 0; // narrowed to what fits
-                    }
-                    if (n <= kList)
-                        n = r.gather(g);
-                    unsigned long long at = 0; // running mass at the word looked for
-                    uint32_t index = 0;
-                    if (n > kList) {
-                        if (stage == ALL) {
-                            if (!weigh) { // a crowd at the cut: weigh every word
-                                weigh = again = true;
-                                break;
-                            }
-                            stage = by_k != kBins ? BY_COUNT : BOTH;
-                            continue;
-                        }
-                        if (stage == BOTH) {
-                            stage = BY_MASS;
-                            continue;
-                        }
-                        n = r.narrow(g, until, base_count, base_mass);
-                        if (n <= kList)
-                            continue;
-                        // words of one value: the place follows from their common mass
-                        value = value_of(g.high);
-                        const unsigned long long each = r.mass_of(r.weight(value));
-                        uint32_t lo = 1, hi = n;
-                        while (lo < hi) {
-                            const uint32_t mid = lo + (hi - lo) / 2;
-                            if (until(base_count + mid, base_mass + mid * each))
-                                hi = mid;
-                            else
-                                lo = mid + 1;
-                        }
-                        at = base_mass + lo * each;
-                        if (stage == DRAW)
-                            nth = lo;
-                    } else if (stage == ALL) {
-                        uint32_t cut = top_k > 0 ? (uint32_t)min((int64_t)n, top_k) : n;
-                        if (top_p < 1.0) {
-                            // without a top-k that cuts, the list may end before the last word that counts
-                            const double want = top_p * (double)(weigh && by_k == kBins ? total : sh.list.mass[cut - 1]);
-                            cut = min(cut, r.listed_before(n, [&](uint32_t i) { return (double)sh.list.mass[i] >= want; }) + 1);
-                        }
-                        if (min_p > 0.0)
-                            cut = min(cut, r.listed_before(n, [&](uint32_t i) {
-                                return !(r.weight(value_of(sh.list.key[i])) >= min_p);
-                            }));
-                        const unsigned long long target = target_of(sh.list.mass[cut - 1]);
-                        const uint32_t i = r.listed_before(cut, [&](uint32_t j) { return sh.list.mass[j] > target; });
-                        drawn = (int32_t)sh.list.index[min(i, cut - 1)];
-                        break;
+            // ALL: everything kept in one list. Otherwise the cuts one by one: by COUNT what top-k
+            // leaves, by MASS what top-p does; DRAW the word. Where top-p's cut is known to a bin the
+            // draw is known to a few: BOTH gathers the words of both.
+            enum { ALL, BY_COUNT, BOTH, BY_MASS, DRAW } stage = ALL;
+            unsigned long long most = total; // mass kept, as far as it is cut
+            Range<Key> g;
+            g.keyed = false;
+            uint32_t base_count = 0;
+            unsigned long long base_mass = 0;
+            if (weigh && sh.count[last] > kList)
+                stage = by_k != kBins ? BY_COUNT : BOTH;
+            for (bool more = true; more;) {
+                uint32_t n = kList + 1;
+                if (!g.keyed) {
+                    if (stage == ALL) {
+                        g.b0 = 0;
+                        g.b1 = g.b2 = last;
+                        n = 0; // tried whatever the counts say: they may be those of the lanes' maxima
                     } else if (stage == BOTH) {
-                        // running masses of the row: whole bins stand in the list, with a gap behind b1
-                        const uint32_t head = g.b1 >= g.b2 ? n : r.listed_before(n, [&](uint32_t i) {
-                            return r.bin_of(value_of(sh.list.key[i])) > (int)g.b1;
-                        });
-                        const unsigned long long base = g.b0 ? sh.mass[g.b0 - 1] : 0;
-                        const unsigned long long skipped = head < n ? base_mass - sh.list.mass[head - 1] : 0;
-                        auto upto = [&](uint32_t i) { return sh.list.mass[i] + (i < head ? base : skipped); };
-                        const uint32_t end = min(r.listed_before(n, [&](uint32_t i) { return (double)upto(i) >= until.reached; }), n - 1);
-                        const unsigned long long target = target_of(min(most, upto(end)));
-                        const uint32_t i = r.listed_before(n, [&](uint32_t j) { return upto(j) > target; });
-                        drawn = (int32_t)sh.list.index[min(i, n - 1)];
-                        break;
+                        until.kind = Until::REACHED;
+                        const uint32_t cut = top_p < 1.0 ? r.first_bin(sh.count, sh.mass, until) : kBins;
+                        if (min_p > 0.0)
+                            most = min(most, own);
+                        if (cut == kBins || (cut ? sh.mass[cut - 1] : 0) >= most) {
+                            stage = DRAW; // top-p takes nothing away
+                            continue;
+                        }
+                        base_mass = cut ? sh.mass[cut - 1] : 0;
+                        until.kind = Until::PASSED;
+                        until.passed = target_of(max(base_mass, 1ull));
+                        g.b0 = r.first_bin(sh.count, sh.mass, until);
+                        until.passed = target_of(min(most, sh.mass[cut]));
+                        g.b1 = r.first_bin(sh.count, sh.mass, until);
+                        g.b2 = cut;
+                        n = count_of(g.b0, g.b1) + count_of(cut, cut);
                     } else {
-                        const uint32_t i = min(r.listed_before(n, [&](uint32_t j) {
-                            return until(base_count + j + 1, base_mass + sh.list.mass[j]);
-                        }), n - 1);
-                        at = base_mass + sh.list.mass[i];
-                        index = sh.list.index[i];
-                        __syncthreads();
+                        until.kind = stage == BY_COUNT ? Until::COUNT : stage == BY_MASS ? Until::REACHED : Until::PASSED;
+                        until.passed = target_of(most);
+                        g.b0 = g.b1 = g.b2 = r.first_bin(sh.count, sh.mass, until);
+                        base_count = g.b2 ? sh.count[g.b2 - 1] : 0;
+                        base_mass = g.b2 ? sh.mass[g.b2 - 1] : 0;
+                        n = count_of(g.b2, g.b2);
                     }
-                    // one cut further
-                    g.keyed = false;
-                    if (stage == BY_COUNT) {
-                        most = at;
-                        until.reached = top_p * (double)most;
-                        stage = BOTH;
-                    } else if (stage == BY_MASS) {
-                        most = min(most, at);
-                        stage = DRAW;
-                    } else {
-                        drawn = (int32_t)index;
-                        more = false;
+                } else {
+                    n = 0; // narrowed to what fits
+                }
+                if (n <= kList)
+                    n = r.gather(g);
+                unsigned long long at = 0; // running mass at the word looked for
+                uint32_t index = 0;
+                if (n > kList) {
+                    if (stage == ALL) {
+                        if (!weigh) { // a crowd at the cut: weigh every word
+                            weigh = again = true;
+                            break;
+                        }
+                        stage = by_k != kBins ? BY_COUNT : BOTH;
+                        continue;
                     }
+                    if (stage == BOTH) {
+                        stage = BY_MASS;
+                        continue;
+                    }
+                    n = r.narrow(g, until, base_count, base_mass);
+                    if (n <= kList)
+                        continue;
+                    // words of one value: the place follows from their common mass
+                    value = value_of(g.high);
+                    const unsigned long long each = r.mass_of(r.weight(value));
+                    uint32_t lo = 1, hi = n;
+                    while (lo < hi) {
+                        const uint32_t mid = lo + (hi - lo) / 2;
+                        if (until(base_count + mid, base_mass + mid * each))
+                            hi = mid;
+                        else
+                            lo = mid + 1;
+                    }
+                    at = base_mass + lo * each;
+                    if (stage == DRAW)
+                        nth = lo;
+                } else if (stage == ALL) {
+                    uint32_t cut = top_k > 0 ? (uint32_t)min((int64_t)n, top_k) : n;
+                    if (top_p < 1.0) {
+                        // without a top-k that cuts, the list may end before the last word that counts
+                        const double want = top_p * (double)(weigh && by_k == kBins ? total : sh.list.mass[cut - 1]);
+                        cut = min(cut, r.listed_before(n, [&](uint32_t i) { return (double)sh.list.mass[i] >= want; }) + 1);
+                    }
+                    if (min_p > 0.0)
+                        cut = min(cut, r.listed_before(n, [&](uint32_t i) {
+                            return !(r.weight(value_of(sh.list.key[i])) >= min_p);
+                        }));
+                    const unsigned long long target = target_of(sh.list.mass[cut - 1]);
+                    const uint32_t i = r.listed_before(cut, [&](uint32_t j) { return sh.list.mass[j] > target; });
+                    drawn = (int32_t)sh.list.index[min(i, cut - 1)];
+                    break;
+                } else if (stage == BOTH) {
+                    // running masses of the row: whole bins stand in the list, with a gap behind b1
+                    const uint32_t head = g.b1 >= g.b2 ? n : r.listed_before(n, [&](uint32_t i) {
+                        return r.bin_of(value_of(sh.list.key[i])) > (int)g.b1;
+                    });
+                    const unsigned long long base = g.b0 ? sh.mass[g.b0 - 1] : 0;
+                    const unsigned long long skipped = head < n ? base_mass - sh.list.mass[head - 1] : 0;
+                    auto upto = [&](uint32_t i) { return sh.list.mass[i] + (i < head ? base : skipped); };
+                    const uint32_t end = min(r.listed_before(n, [&](uint32_t i) { return (double)upto(i) >= until.reached; }), n - 1);
+                    const unsigned long long target = target_of(min(most, upto(end)));
+                    const uint32_t i = r.listed_before(n, [&](uint32_t j) { return upto(j) > target; });
+                    drawn = (int32_t)sh.list.index[min(i, n - 1)];
+                    break;
+                } else {
+                    const uint32_t i = min(r.listed_before(n, [&](uint32_t j) {
+                        return until(base_count + j + 1, base_mass + sh.list.mass[j]);
+                    }), n - 1);
+                    at = base_mass + sh.list.mass[i];
+                    index = sh.list.index[i];
+                    __syncthreads();
+                }
+                // one cut further
+                g.keyed = false;
+                if (stage == BY_COUNT) {
+                    most = at;
+                    until.reached = top_p * (double)most;
+                    stage = BOTH;
+                } else if (stage == BY_MASS) {
+                    most = min(most, at);
+                    stage = DRAW;
+                } else {
+                    drawn = (int32_t)index;
+                    more = false;
                 }
             }
         }
-        __syncthreads();
-        if (nth)
-            drawn = (int32_t)r.nth_of_value(value, nth);
-        if (tid == 0)
-            p.out[row] = drawn;
-        __syncthreads(); // the next row writes the shared memory again
     }
+    __syncthreads();
+    if (nth)
+        drawn = (int32_t)r.nth_of_value(value, nth);
+    if (tid == 0)
+        p.out[row] = drawn;
 }
 
 // Slices per row and the workspace for what they leave: host arithmetic on the sizes and on what the
@@ -964,7 +959,8 @@ int run(const cnh_sample_tokens_args* a, const Plan& q, hipStream_t st) {
         slice_top_kernel<T><<<grid, kThreads, 0, st>>>(p);
         slice_weigh_kernel<T><<<grid, kThreads, 0, st>>>(p);
     }
-    sample_kernel<T><<<(unsigned)std::min<int64_t>(p.rows, 1 << 20), kThreads, 0, st>>>(p);
+    for (p.first_row = 0; p.first_row < p.rows; p.first_row += 1 << 20) // a grid takes fewer than 2^32 lanes
+        sample_kernel<T><<<(unsigned)std::min<int64_t>(p.rows - p.first_row, 1 << 20), kThreads, 0, st>>>(p);
     CNH_HIP(hipGetLastError());
     return 0;
 }
