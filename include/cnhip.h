@@ -491,10 +491,12 @@ int cnh_fill_uniform_tile(double* out, int ndims, const int64_t* ext, const int6
  * other (-2) except where it says so, each operand taken from its first element to its last;
  * `lengths` (device, one per sequence) holds how many of its `length` tokens a sequence has, values
  * outside [0, length] being held to it: rows of y behind them are zeros, whatever x holds there, and
- * the state is that behind the last token that counts. */
+ * the state is that behind the last token that counts. Rows, batches and lengths are below 2^31, channels
+ * below 2^28 (below 2^24 in the scan); more is refused (-3). */
 
 /* r = x + residual; y = r / sqrt(mean over the row of r^2 + eps) * weight. residual, residual_out and
- * weight (ones) are optional; residual_out receives r and may be the residual itself. */
+ * weight (ones) are optional; residual_out receives r and may be the residual itself. The squares are
+ * summed in the rows' own type: a sum beyond its range makes a row of zeros, as 1 / infinity does. */
 typedef struct cnh_rms_norm_args {
     int32_t dtype;
     int64_t rows, cols;
@@ -542,7 +544,8 @@ int cnh_short_convolution(const cnh_short_convolution_args* a, cnh_stream s);
  * (device, 16-byte aligned, undefined contents before and after) then holds the bytes
  * cnh_state_scan_workspace asks for (it looks at the type and the sizes alone and needs no device).
  * Calls that may run at the same time need workspaces of their own, captured graphs among them. The
- * cut depends on the sizes alone; an output's last bits can differ between batch sizes. */
+ * cut depends on the sizes alone; an output's last bits can differ between batch sizes. Tokens of a
+ * sequence are less than 2 GiB apart in every operand (-3). */
 typedef struct cnh_state_scan_args {
     int32_t dtype, softplus;
     int64_t batch, length, channels, states;

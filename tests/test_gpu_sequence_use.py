@@ -240,6 +240,16 @@ def test_more_sequences_and_rows_than_a_grid_holds(dev):
         got = fetch(p.value + first * cols * 4, cols, cols, 3)
         close(got, np.repeat(y, 3, axis=0), np.repeat(ey, 3, axis=0), f"norm, rows from {first}")
     L.check(L.lib.cnh_free(p))
+    n, D, K = 4 * 65535 * 8 + 21, 3, 3                       # one long sequence through the convolution
+    x = np.random.default_rng(4).standard_normal((1, n, D)).astype(np.float32)
+    w = np.random.default_rng(5).standard_normal((K, D)).astype(np.float32)
+    dx, dw, dy, st = dev.array(x), dev.array(w), dev.array(np.full((1, n, D), 7, np.float32)), dev.array(np.zeros((1, K - 1, D), np.float32))
+    L.check(L.lib.cnh_short_convolution(C.byref(L.ShortConvolution(
+        L.F32, 0, K, 1, n, D, dx.ptr, n * D, D, dw.ptr, None, None, st.ptr, None, dy.ptr, n * D, D)), None))
+    y, after, ey = R.short_convolution(x, w, None, None, None, False, u)
+    close(dy.get(), y, ey, "convolution of a long sequence")
+    assert np.array_equal(st.get().astype(np.float64), after)
+    dev.free_all()
     logits = dev.array(np.array([0.0, 1.0, 2.0, -1.0], np.float32))
     un = np.random.default_rng(3).random(rows)
     du, out = dev.array(un), dev.array(np.full(rows, -9, np.int32))

@@ -98,12 +98,17 @@ NAN = float("nan")
     (conv, dict(state_out=4 * BIG + 32), -2, "without being the same"),
     (conv, dict(state_out=6 * BIG), -2, "state_out overlaps lengths"),
     (conv, dict(lengths=6 * BIG + 2), -2, "not aligned"),
+    (conv, dict(channels=1 << 28), -3, "channels"),
+    (conv, dict(length=1 << 31), -3, "length"),
     (scan, dict(dtype=L.I64), -2, "element type"),
     (scan, dict(states=0), -3, "states"),
     (scan, dict(states=257), -3, "states"),
     (scan, dict(softplus=3), -2, "softplus"),
     (scan, dict(batch=-1), -2, "batch"),
     (scan, dict(channels=1 << 24), -3, "channels"),
+    (scan, dict(batch=1, length=2, x=100 * BIG, x_stride=1 << 29), -3, "less than 2 GiB"),
+    (scan, dict(batch=1, length=2, C=100 * BIG, C_stride=1 << 29), -3, "less than 2 GiB"),
+    (scan, dict(dtype=L.F64, batch=1, length=2, y=100 * BIG, y_stride=1 << 28), -3, "less than 2 GiB"),
     (scan, dict(A=None), -2, "null"),
     (scan, dict(delta=None), -2, "null"),
     (scan, dict(B_stride=-1), -2, "stride of B"),
