@@ -21,8 +21,11 @@
 // Few rows whose every word has to be weighed are cut into slices: a pass for the slices' maxima, one that
 // adds their weights up bin by bin in the workspace, and the row's own workgroup goes on from there.
 //
-// Bound by memory for many rows (one workgroup per row, the passes behind the first come from the
-// caches) and by the length of one row's passes for few.
+// A row is one workgroup's: what bounds it is the 62 GB/s that one CU reads, the 64-bit arithmetic of the
+// weighing, and some twenty short phases that each wait for their instructions. One row of 131072 fp32
+// words with a top-k of 50: 18.4 us (two passes of 4.2 us are memory). 256 rows of 50021, settings mixed:
+// 34.8 us, the time of a row that has to be weighed; 256 of 1000 words, sorted whole: 12.8 us. One row of
+// 131072 without a top-k, in 16 slices: 4 + 6 + 15.5 us.
 #include "sequence.h"
 
 #include <algorithm>

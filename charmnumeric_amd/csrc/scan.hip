@@ -16,7 +16,12 @@
 // piece of the sequence is summed up by the state it leaves when it starts from zero and by the sum of
 // its steps (its decay is exp(A sum s)); a short pass over the pieces gives each its first state, and
 // all pieces then run at once. That costs the exponentials twice, which is why it is left out as soon
-// as the batch fills the device by itself.
+// as half the vector units have a wavefront each, and for prompts below 96 tokens.
+//
+// Prompts are bound by vector issue: a state of a token takes an exponential of 8.5 cycles and three to four
+// operations of 4.3 to 5. One prompt of 8192 tokens, 2048 channels and 16 fp32 states, in 128 pieces: 59 us for
+// what the pieces leave, 11 for their first states, 76 for the scan, vector issue busy 85 % of the time.
+// One token of 128 x 4096 channels is bound by the states: 13.4 us, 75 MB at 5.6 TB/s.
 #include "sequence.h"
 
 #include <algorithm>
@@ -408,11 +413,11 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
     }
 }
 
-// The state each piece starts from, in place of the one it leaves: 64 channels of one state per
-// workgroup, up to kSegments x GROUP pieces a round (as many segments as the pieces need). A lane loads its GROUP pieces at once, folds them to one,
-// takes what the segments before it leave from shared memory and walks its pieces again in registers;
-// one lane per channel that walks all pieces by itself waits for memory once per GROUP of them instead
-// (128 pieces of 2048 x 16 fp32 states: 22.5 us).
+// The state each piece starts from, in place of the one it leaves: 64 channels of one state per workgroup,
+// up to kSegments x GROUP pieces a round (as many segments as the pieces need). A lane loads its GROUP
+// pieces at once, folds them to one, takes what the segments before it leave from shared memory and walks
+// its pieces again in registers. 128 pieces of 2048 x 16 fp32 states: 10.7 us; with one lane per channel
+// that walks all pieces by itself and waits for memory once per GROUP of them 22.5 us.
 constexpr int kSegments = 8, kGroup = 8;
 template <typename T>
 __global__ __launch_bounds__(64 * kSegments) void carry_kernel(ScanParams<T> p) {
@@ -465,7 +470,7 @@ __global__ __launch_bounds__(64 * kSegments) void carry_kernel(ScanParams<T> p) 
 
 // One token per sequence. The states are what moves: they are read and written once as 16-byte
 // accesses, a lane keeps its channel's A through the sequences of its slice, and the next sequence's
-// operands are on their way while the present one is worked on.
+// operands are on their way while the present one is worked on (128 x 4096 x 16 fp32 states: 13.4 us).
 template <typename T, int NPL, int S, bool FULL>
 __global__ __launch_bounds__(256) void token_kernel(ScanParams<T> p) {
     const uint32_t lane = blockIdx.x * 256 + threadIdx.x;
