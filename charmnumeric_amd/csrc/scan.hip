@@ -58,11 +58,13 @@ struct ScanParams {
 
 // exp(s A) with what depends on A alone taken out of the loop: the 32-bit form is one multiplication
 // and the hardware's base-2 exponential (1 ulp); rounding A log2(e) shifts the exponent by at most
-// |s A| 2^-24, which the decay's own size makes harmless.
+// |s A| 2^-24, which the decay's own size makes harmless. The 64-bit form is the same with a polynomial for
+// the exponential, which wants a finite argument: steps and rates beyond 1e150 are held to it.
 __device__ __forceinline__ float rate_of(float a) { return a * 1.44269504088896341f; }
-__device__ __forceinline__ double rate_of(double a) { return a; }
+__device__ __forceinline__ double held(double v) { return fmin(fmax(v, -1e150), 1e150); }
+__device__ __forceinline__ double rate_of(double a) { return a != a ? a : held(a * 1.4426950408889634); }
 __device__ __forceinline__ float decay(float s, float rate) { return __builtin_amdgcn_exp2f(s * rate); }
-__device__ __forceinline__ double decay(double s, double rate) { return exp(s * rate); }
+__device__ __forceinline__ double decay(double s, double rate) { return exp2_of(held(s) * rate); }
 
 // log(1 + e^v). In 32 bits log(u) e / (u - 1) with u = 1 + e^v rounded: the rounding of u cancels.
 __device__ __forceinline__ float softplus(float v) {
@@ -71,7 +73,32 @@ __device__ __forceinline__ float softplus(float v) {
     const float r = d == 0.0f ? e : l * (e * __builtin_amdgcn_rcpf(d));
     return v > 20.0f ? v : r;
 }
-__device__ __forceinline__ double softplus(double v) { return v > 40.0 ? v : log1p(exp(v)); }
+// In 64 bits max(v, 0) + log(1 + e) with e = e^-|v|, log(1 + e) = 2 atanh(e / (e + 2)) for small e and
+// log 2 + 2 atanh((e - 1) / (e + 3)) above sqrt(2) - 1, so that the series' argument stays within 0.1716: ten
+// terms leave 2^-58 of it.
+__device__ __forceinline__ double softplus(double v) {
+    const double e = exp_of_minus(v);
+    const bool upper = e > 0.41421356237309503;
+    const double num = upper ? e - 1.0 : e, den = e + (upper ? 3.0 : 2.0);
+    double r = __builtin_amdgcn_rcp(den); // and Newton's steps
+    r = fma(fma(-den, r, 1.0), r, r);
+    r = fma(fma(-den, r, 1.0), r, r);
+    double q = num * r;
+    q = fma(fma(-den, q, num), r, q);
+    const double z = q * q;
+    double t = 1.0 / 21;
+    t = fma(t, z, 1.0 / 19);
+    t = fma(t, z, 1.0 / 17);
+    t = fma(t, z, 1.0 / 15);
+    t = fma(t, z, 1.0 / 13);
+    t = fma(t, z, 1.0 / 11);
+    t = fma(t, z, 1.0 / 9);
+    t = fma(t, z, 1.0 / 7);
+    t = fma(t, z, 1.0 / 5);
+    t = fma(t, z, 1.0 / 3);
+    const double l = fma(2.0 * q, z * t, 2.0 * q) + (upper ? 0.693147180559945309 : 0.0);
+    return (v < 0.0 ? 0.0 : v) + l;
+}
 
 // Sum over S neighbouring lanes, in every one of them.
 template <int S, typename T>
