@@ -161,8 +161,17 @@ struct ScalarRow<64> {
     typedef uint32_t type __attribute__((ext_vector_type(16), aligned(4)));
 };
 
-// NPL states (n0 .. n0 + NPL) of one token's B or C. FULL: all of them exist, the rows of A and of the
-// states are aligned for wide accesses and, with S > 1, those of B and C too.
+// The states of a lane: NPL one behind the other from n0 on when FULL (all of them exist, the rows of A and of
+// the states are aligned for wide accesses and, with S > 1, those of B and C too); every S-th from n0 on
+// otherwise, so that the lanes of a channel read neighbouring elements.
+template <int S, bool FULL>
+constexpr int STEP = FULL ? 1 : S;
+template <int NPL, int S, bool FULL>
+__device__ __forceinline__ int first_state(uint32_t lane) {
+    return (int)(lane % S) * (FULL ? NPL : 1);
+}
+
+// Those of one token's B or C.
 template <typename T, int NPL, int S, bool FULL>
 __device__ __forceinline__ void load_states(T (&v)[NPL], const T* row, int n0, int states) {
     if constexpr (S == 1) {
@@ -182,51 +191,54 @@ __device__ __forceinline__ void load_states(T (&v)[NPL], const T* row, int n0, i
         // the last state again for those that do not exist: no branches between the loads
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
-            const T at = row[min(n0 + i, states - 1)];
-            v[i] = n0 + i < states ? at : T(0);
+            const int n = n0 + i * STEP<S, FULL>;
+            const T at = row[min(n, states - 1)];
+            v[i] = n < states ? at : T(0);
         }
     }
 }
 
-// NPL states of a lane's own channel, from a row of `states` elements.
-template <typename T, int NPL, bool FULL>
+// Those of a lane's own channel, from a row of `states` elements.
+template <typename T, int NPL, int S, bool FULL>
 __device__ __forceinline__ void own_states(Pack<T, NPL>& v, const T* row, int n0, int states) {
     if constexpr (FULL) {
         load_pack(v, row + n0);
     } else {
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
-            v.v[i] = n0 + i < states ? row[n0 + i] : T(0);
+            v.v[i] = n0 + i * STEP<S, FULL> < states ? row[n0 + i * STEP<S, FULL>] : T(0);
     }
 }
 
-template <typename T, int NPL, bool FULL>
+template <typename T, int NPL, int S, bool FULL>
 __device__ __forceinline__ void store_states(const Pack<T, NPL>& v, T* row, int n0, int states) {
     if constexpr (FULL) {
         store_pack(v, row + n0);
     } else {
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
-            if (n0 + i < states)
-                row[n0 + i] = v.v[i];
+            if (n0 + i * STEP<S, FULL> < states)
+                row[n0 + i * STEP<S, FULL>] = v.v[i];
     }
 }
 
 // PARTIAL: what a piece leaves when it starts from zero; otherwise the scan itself.
 template <typename T, int NPL, int S, bool FULL, bool PARTIAL>
 __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
-    constexpr int AHEAD = 4; // tokens whose x, delta and z are on their way while others are worked on
+    // Tokens whose x, delta and z are on their way while others are worked on. With S > 1 their rows of B and
+    // C are loaded together: no more than 64 registers of them.
+    constexpr int AHEAD = S > 1 ? std::min(4, 128 / (NPL * (int)sizeof(T))) : 4;
     const uint32_t lane = blockIdx.x * 64 + threadIdx.x; // below 2^28: 16 lanes for each of 2^24 channels
     const uint32_t d_own = lane / S;
     const bool live = d_own < (uint32_t)p.channels;
     // lanes past the last channel work on the last one and store nothing: the wavefront stays whole
     const uint32_t d = live ? d_own : (uint32_t)p.channels - 1;
-    const int n0 = (int)(lane % S) * NPL;
+    const int n0 = first_state<NPL, S, FULL>(lane);
     const uint32_t off = d * (uint32_t)sizeof(T);
     const bool first = n0 == 0;
     const int64_t piece = blockIdx.y;
     Pack<T, NPL> rate;
-    own_states<T, NPL, FULL>(rate, p.A + (int64_t)d * p.states, n0, p.states);
+    own_states<T, NPL, S, FULL>(rate, p.A + (int64_t)d * p.states, n0, p.states);
 #pragma unroll
     for (int i = 0; i < NPL; ++i)
         rate.v[i] = rate_of(rate.v[i]);
@@ -249,9 +261,9 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
         if (p.pieces > 1) {
 #pragma unroll
             for (int i = 0; i < NPL; ++i)
-                h.v[i] = FULL || n0 + i < p.states ? slot[(int64_t)i * p.channels] : T(0);
+                h.v[i] = FULL || n0 + i * STEP<S, FULL> < p.states ? slot[(int64_t)(i * STEP<S, FULL>) * p.channels] : T(0);
         } else if (p.state_in) {
-            own_states<T, NPL, FULL>(h, p.state_in + (b * p.channels + d) * p.states, n0, p.states);
+            own_states<T, NPL, S, FULL>(h, p.state_in + (b * p.channels + d) * p.states, n0, p.states);
         }
     }
     T steps = 0;
@@ -425,8 +437,8 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
         if (live) {
 #pragma unroll
             for (int i = 0; i < NPL; ++i)
-                if (FULL || n0 + i < p.states)
-                    slot[(int64_t)i * p.channels] = h.v[i];
+                if (FULL || n0 + i * STEP<S, FULL> < p.states)
+                    slot[(int64_t)(i * STEP<S, FULL>) * p.channels] = h.v[i];
             if (first)
                 p.steps[(b * p.pieces + piece) * p.channels + d] = steps;
         }
@@ -435,7 +447,7 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
             for (int64_t t = std::max(begin, end); t < stop; ++t)
                 at(on(yp, t * (int64_t)p.y_s), off) = T(0);
         if (p.state_out && piece == p.pieces - 1 && live) {
-            store_states<T, NPL, FULL>(h, p.state_out + (b * p.channels + d) * p.states, n0, p.states);
+            store_states<T, NPL, S, FULL>(h, p.state_out + (b * p.channels + d) * p.states, n0, p.states);
         }
     }
 }
@@ -504,10 +516,10 @@ __global__ __launch_bounds__(256) void token_kernel(ScanParams<T> p) {
     const uint32_t d_own = lane / S;
     const bool live = d_own < (uint32_t)p.channels;
     const uint32_t d = live ? d_own : (uint32_t)p.channels - 1;
-    const int n0 = (int)(lane % S) * NPL;
+    const int n0 = first_state<NPL, S, FULL>(lane);
     const int64_t begin = blockIdx.y * p.piece, end = std::min(begin + p.piece, p.batch);
     Pack<T, NPL> rate;
-    own_states<T, NPL, FULL>(rate, p.A + (int64_t)d * p.states, n0, p.states);
+    own_states<T, NPL, S, FULL>(rate, p.A + (int64_t)d * p.states, n0, p.states);
 #pragma unroll
     for (int i = 0; i < NPL; ++i)
         rate.v[i] = rate_of(rate.v[i]);
@@ -526,7 +538,7 @@ __global__ __launch_bounds__(256) void token_kernel(ScanParams<T> p) {
         load_states<T, NPL, S, FULL>(o.C, p.C + b * p.C_bs, n0, p.states);
         o.h = Pack<T, NPL>{};
         if (p.state_in)
-            own_states<T, NPL, FULL>(o.h, p.state_in + (b * p.channels + d) * p.states, n0, p.states);
+            own_states<T, NPL, S, FULL>(o.h, p.state_in + (b * p.channels + d) * p.states, n0, p.states);
     };
     Operands next;
     fetch(begin, next);
@@ -552,7 +564,7 @@ __global__ __launch_bounds__(256) void token_kernel(ScanParams<T> p) {
             if (n0 == 0)
                 (p.y + b * p.y_bs)[d] = out;
             if (p.state_out)
-                store_states<T, NPL, FULL>(o.h, p.state_out + (b * p.channels + d) * p.states, n0, p.states);
+                store_states<T, NPL, S, FULL>(o.h, p.state_out + (b * p.channels + d) * p.states, n0, p.states);
         }
     }
 }
@@ -583,7 +595,7 @@ Plan plan_of(const cnh_state_scan_args* a) {
     // pieces of 32 tokens that the call could be cut into would not fill the device with many.
     // For 33 to 64 states few are faster always (64 states, 2048 channels, sixteen a lane and four: 16 x 100
     // tokens 116 and 97 us in fp32, 397 and 311 in fp64; 4 x 300 tokens 139 and 102, 478 and 242).
-    const int many = N <= 8 ? 8 : N <= 16 || N > 32 ? 16 : 32;
+    const int many = N <= 8 || (N > 64 && N <= 128) ? 8 : N <= 16 || N > 128 ? 16 : 32;
     q.npl = many;
     if (N <= 64 && (N > 32 || N <= 4 || L <= 1 || waves(lanes(many)) * std::max<int64_t>(1, L / 32) < 2 * kUnits))
         q.npl = 4;
@@ -599,7 +611,8 @@ Plan plan_of(const cnh_state_scan_args* a) {
         // Measured with 300 tokens of 2048 fp32 channels, 16 states: 16 sequences (512 wavefronts) 120 us
         // uncut, 95 us in 8 pieces; 24 sequences (768) 129 us uncut, 134 us in 3. With 256 channels of
         // 2 sequences: 64 tokens 20 us uncut, 22 us in 4 pieces; 128 tokens 29 and 22 us.
-        if (w <= kUnits / 2 && w > 0 && L >= 96)
+        const bool early = q.lanes == 1 && N == q.npl && N * dtype_size(a->dtype) <= 64;
+        if (w <= (early ? kUnits / 2 : kUnits * 5 / 8) && w > 0 && L >= 96)
             q.pieces = (int)std::min(4 * kUnits / w, L / 16);
         q.piece = (L + q.pieces - 1) / q.pieces;
         q.pieces = (int)((L + q.piece - 1) / q.piece);
@@ -680,14 +693,10 @@ int run(const cnh_state_scan_args* a, const Plan& q, hipStream_t st) {
         }
     }
     if (q.npl == 8)
-        return launch_full<T, 8, 1>(p, wide, st);
-    if (q.npl == 32)
-        return launch_full<T, 32, 1>(p, wide, st);
-    switch (q.lanes) {
-    case 1: return launch_full<T, 16, 1>(p, wide, st);
-    case 8: return launch_full<T, 16, 8>(p, wide, st);
-    default: return launch_full<T, 16, 16>(p, wide, st);
-    }
+        return q.lanes == 1 ? launch_full<T, 8, 1>(p, wide, st) : launch_full<T, 8, 16>(p, wide, st);
+    if (q.npl == 16)
+        return q.lanes == 1 ? launch_full<T, 16, 1>(p, wide, st) : launch_full<T, 16, 16>(p, wide, st);
+    return launch_full<T, 32, 1>(p, wide, st);
 }
 
 int check_sizes(const cnh_state_scan_args* a, const char* call) {
