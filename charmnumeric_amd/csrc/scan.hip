@@ -59,8 +59,11 @@ struct ScanParams {
 // exp(s A) with what depends on A alone taken out of the loop: the 32-bit form is one multiplication
 // and the hardware's base-2 exponential (1 ulp); rounding A log2(e) shifts the exponent by at most
 // |s A| 2^-24, which the decay's own size makes harmless. The 64-bit form is the same with a polynomial for
-// the exponential, which wants a finite argument: steps and rates beyond 1e150 are held to it.
-__device__ __forceinline__ float rate_of(float a) { return a * 1.44269504088896341f; }
+// the exponential, which wants a finite argument: steps and rates beyond 1e150 are held to it. An infinite
+// rate is held to a finite one in 32 bits too, so that no step (pieces behind a sequence's end) is no decay.
+__device__ __forceinline__ float rate_of(float a) {
+    return a != a ? a : fminf(fmaxf(a * 1.44269504088896341f, -3e38f), 3e38f);
+}
 __device__ __forceinline__ double held(double v) { return fmin(fmax(v, -1e150), 1e150); }
 __device__ __forceinline__ double rate_of(double a) { return a != a ? a : held(a * 1.4426950408889634); }
 __device__ __forceinline__ float decay(float s, float rate) { return __builtin_amdgcn_exp2f(s * rate); }
@@ -595,9 +598,15 @@ Plan plan_of(const cnh_state_scan_args* a) {
     // pieces of 32 tokens that the call could be cut into would not fill the device with many.
     // For 33 to 64 states few are faster always (64 states, 2048 channels, sixteen a lane and four: 16 x 100
     // tokens 116 and 97 us in fp32, 397 and 311 in fp64; 4 x 300 tokens 139 and 102, 478 and 242).
+    // A lane whose many are not all there reads B and C element by element: in uncut calls few are faster
+    // with less than a wavefront per unit (22 x 200 tokens of 2048 channels, 12 states: 223 and 113 us in fp32,
+    // 485 and 350 in fp64; 62 x 200 tokens, 10 states: 259 and 292, 592 and 909), and from 17 states on always
+    // (65 x 100 tokens, 20 states: 354 and 282, 1022 and 924).
     const int many = N <= 8 || (N > 64 && N <= 128) ? 8 : N <= 16 || N > 128 ? 16 : 32;
+    const int64_t wm = waves(lanes(many));
+    const bool sparse = N != many && wm > kUnits * 5 / 8 && (N > 16 || wm < kUnits);
     q.npl = many;
-    if (N <= 64 && (N > 32 || N <= 4 || L <= 1 || waves(lanes(many)) * std::max<int64_t>(1, L / 32) < 2 * kUnits))
+    if (N <= 64 && (N > 32 || N <= 4 || L <= 1 || wm * std::max<int64_t>(1, L / 32) < 2 * kUnits || sparse))
         q.npl = 4;
     q.lanes = lanes(q.npl);
     q.pieces = 1;
@@ -610,7 +619,9 @@ Plan plan_of(const cnh_state_scan_args* a) {
     } else {
         // Measured with 300 tokens of 2048 fp32 channels, 16 states: 16 sequences (512 wavefronts) 120 us
         // uncut, 95 us in 8 pieces; 24 sequences (768) 129 us uncut, 134 us in 3. With 256 channels of
-        // 2 sequences: 64 tokens 20 us uncut, 22 us in 4 pieces; 128 tokens 29 and 22 us.
+        // 2 sequences: 64 tokens 20 us uncut, 22 us in 4 pieces; 128 tokens 29 and 22 us. Where B and C do
+        // not travel ahead in scalar registers a lone wavefront waits for them: 17 sequences (544 wavefronts)
+        // of 32 states 309 us uncut, 181 in 7 pieces; fp64 12 states 723 and 430.
         const bool early = q.lanes == 1 && N == q.npl && N * dtype_size(a->dtype) <= 64;
         if (w <= (early ? kUnits / 2 : kUnits * 5 / 8) && w > 0 && L >= 96)
             q.pieces = (int)std::min(4 * kUnits / w, L / 16);
@@ -623,12 +634,13 @@ Plan plan_of(const cnh_state_scan_args* a) {
 
 template <typename T, int NPL, int S, bool FULL>
 int launch(ScanParams<T> p, hipStream_t st) {
-    if (p.length == 1) {
-        const dim3 grid((unsigned)((p.channels * S + 255) / 256), (unsigned)((p.batch + p.piece - 1) / p.piece));
-        token_kernel<T, NPL, S, FULL><<<grid, 256, 0, st>>>(p);
-        CNH_HIP(hipGetLastError());
-        return 0;
-    }
+    if constexpr (NPL == 4 || S == 16) // what single tokens take
+        if (p.length == 1) {
+            const dim3 grid((unsigned)((p.channels * S + 255) / 256), (unsigned)((p.batch + p.piece - 1) / p.piece));
+            token_kernel<T, NPL, S, FULL><<<grid, 256, 0, st>>>(p);
+            CNH_HIP(hipGetLastError());
+            return 0;
+        }
     // one wavefront per workgroup: few long-running wavefronts spread evenly over the device
     const unsigned gx = (unsigned)((p.channels * S + 63) / 64);
     for (p.first_batch = 0; p.first_batch < p.batch; p.first_batch += 65535) { // what a grid takes

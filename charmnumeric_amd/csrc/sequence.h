@@ -175,9 +175,12 @@ __device__ __forceinline__ int64_t tokens_of(const int32_t* lengths, int64_t b, 
 
 // 2^t for finite t, to an ulp: 2^k times a polynomial in t - k for the nearest integer k, the interpolation of
 // 2^f at the Chebyshev nodes of [-1/2, 1/2] (2^-55 off at most, its rounded coefficients included). The
-// library's exponential spends a third of its instructions on its range; here k and the final scaling
-// saturate by themselves.
+// library's exponential spends a third of its instructions on its range; here the conversion of k saturates,
+// and one instruction more holds the scaling to exponents that it takes (not to the lowest integer).
 __device__ __forceinline__ double exp2_of(double t) {
+// t - k without the product behind t drawn into it: its rounding error is no part of f, and would be far from
+// small where t is large.
+#pragma clang fp contract(off)
     const double k = rint(t), f = t - k;
     double p = 4.4558179083360645e-10;
     p = fma(p, f, 7.074194297288521e-09);
@@ -193,7 +196,7 @@ __device__ __forceinline__ double exp2_of(double t) {
     p = fma(p, f, 1.0);
     int n; // the instruction itself: a C++ cast says nothing about what does not fit
     asm("v_cvt_i32_f64 %0, %1" : "=v"(n) : "v"(k));
-    return __builtin_amdgcn_ldexp(p, n);
+    return __builtin_amdgcn_ldexp(p, max(min(n, 4096), -4096));
 }
 // e^-|x|; 0 for NaN.
 __device__ __forceinline__ double exp_of_minus(double x) {

@@ -8,7 +8,7 @@ import pytest
 from charmnumeric_amd import _lib as L
 from tests import helpers as H
 from tests import sequence_reference as R
-from tests.test_gpu_sequence import close, scan_inputs
+from tests.test_gpu_sequence import close, scan_call, scan_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -284,4 +284,63 @@ def test_padding_and_memory_behind_the_sequences(dev):
     assert np.array_equal(h.get()[1], q["state"][1])
     for k, v in q.items():
         assert np.array_equal(d[k].get(), v), k
+    dev.free_all()
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("B,n,N", [
+    (2048, 33, 5), (2048, 33, 8), (2048, 33, 12), (2048, 33, 16), (2048, 33, 20), (2048, 33, 32), (2048, 33, 40),
+    (256, 256, 5), (256, 256, 8), (256, 256, 12), (256, 256, 16), (256, 256, 20), (256, 256, 32),
+    (600, 130, 6), (600, 130, 12), (600, 130, 16), (600, 130, 32), (700, 130, 7), (700, 130, 16), (700, 130, 24),
+])
+def test_scan_of_many_sequences(dev, dtype, B, n, N):
+    """Batches that fill the device, with one and with several states a lane, whole and cut: one sequence
+    repeated by a stride of zero, every one of them with a state of its own."""
+    D, u = 64, R.half_step(dtype)
+    q = scan_inputs(dtype, 1, n, D, N, n + N)
+    one, rep = {k: dev.array(v) for k, v in q.items()}, dev.array(np.repeat(q["state"], B, axis=0))
+    dy = dev.array(np.full((B, n, D), 7, dtype))
+    a = L.StateScan(L.F32 if dtype == np.float32 else L.F64, 1, B, n, D, N, one["x"].ptr, 0, D, one["delta"].ptr, 0, D,
+                    one["z"].ptr, 0, D, one["A"].ptr, one["Bm"].ptr, 0, N, one["Cm"].ptr, 0, N, one["skip"].ptr,
+                    one["delta_bias"].ptr, rep.ptr, rep.ptr, None, dy.ptr, n * D, D)
+    a.workspace_bytes = L.check(L.lib.cnh_state_scan_workspace(C.byref(a)))
+    if a.workspace_bytes:
+        a.workspace = dev.array(np.full(a.workspace_bytes // 4, np.nan, np.float32)).ptr
+    L.check(L.lib.cnh_state_scan(C.byref(a), None))
+    y, h, ey, eh = R.state_scan(**q, lengths=None, softplus=True, u=u, piece=64)
+    got, hs = dy.get(), rep.get()
+    assert (got == got[:1]).all() and (hs == hs[:1]).all()
+    close(got[:1], y, ey, "scan")
+    close(hs[:1], h, eh, "state")
+    dev.free_all()
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("n,N", [(1, 16), (40, 16), (40, 13), (40, 100), (700, 8)])
+def test_scan_of_infinities_and_nan(dev, dtype, n, N):
+    """A rate of -infinity forgets at once, whatever came before; what is no number stays in its channel and
+    behind its token. The longest prompt is padded by more than a piece of its cut."""
+    D, u = 70, R.half_step(dtype)
+    last = n if n < 700 else n - 50
+    lengths = None if last == n else [last]
+    q = scan_inputs(dtype, 1, n, D, N, n * N)
+    q["A"][:, 0] = -1e6                                       # decays that are zero already
+    q["delta_bias"][:] = 1.0                                  # steps of 0.1 and more
+    y, h, ey, eh = R.state_scan(**q, lengths=lengths, softplus=True, u=u, piece=64)
+    q["A"][:, 0] = -np.inf
+    bad = n // 2
+    q["x"][0, bad, 5] = np.nan
+    q["delta"][0, bad, 66] = np.nan
+    q["A"][9, N - 1] = np.nan
+    q["z"][0, bad, 12] = np.nan
+    got, out, _ = scan_call(dev, dtype, q, lengths, True)
+    for d in (5, 66, 9):
+        first = 0 if d == 9 else bad
+        assert np.isnan(got[0, first:last, d]).all()
+        assert np.isnan(out[0, d]).all() if d != 9 else np.isnan(out[0, d, N - 1])
+        got[0, first:last, d], out[0, d] = y[0, first:last, d], h[0, d]
+    assert np.isnan(got[0, bad, 12])
+    got[0, bad, 12] = y[0, bad, 12]
+    close(got, y, ey, "scan")
+    close(out, h, eh, "state")
     dev.free_all()
