@@ -16,7 +16,8 @@
 // piece of the sequence is summed up by the state it leaves when it starts from zero and by the sum of
 // its steps (its decay is exp(A sum s)); a short pass over the pieces gives each its first state, and
 // all pieces then run at once. That costs the exponentials twice, which is why it is left out as soon
-// as half the vector units have a wavefront each, and for prompts below 96 tokens.
+// as half the vector units have a wavefront each (five eighths where B and C cannot be sent for ahead), and
+// for prompts below 96 tokens.
 //
 // Prompts are bound by vector issue: a state of a token takes an exponential of 8.5 cycles and three to four
 // operations of 4.3 to 5. One prompt of 8192 tokens, 2048 channels and 16 fp32 states, in 128 pieces: 59 us for
