@@ -70,6 +70,27 @@ __device__ __forceinline__ double rate_of(double a) { return a != a ? a : held(a
 __device__ __forceinline__ float decay(float s, float rate) { return __builtin_amdgcn_exp2f(s * rate); }
 __device__ __forceinline__ double decay(double s, double rate) { return exp2_of(held(s) * rate); }
 
+// The decay of many tokens, 2^f 2^k: it can leave the type's range where the state does not (states that grow from
+// nothing or little, or large ones over a long piece). 2^f h scaled by 2^k leaves nothing at nothing, and the range
+// only where the state itself is out of it. f is taken from the product before its rounding; exponents beyond `far`
+// bring every number of the type out of its range.
+template <typename T>
+struct LongDecay {
+    T part; // 2^f, |f| <= 1/2
+    int k;
+    __device__ __forceinline__ T operator()(T h) const { return ldexp(part * h, k); }
+};
+template <typename T>
+__device__ __forceinline__ LongDecay<T> long_decay(T s, T rate) {
+    constexpr T far = sizeof(T) == 4 ? T(600) : T(4400);
+    const T t = s * rate, k = fmin(fmax(rint(t), -far), far);   // -far for no number, which f hands on
+    const T f = fabs(t) > far ? T(0) : fma(s, rate, -k);
+    if constexpr (sizeof(T) == 4)
+        return {__builtin_amdgcn_exp2f(f), (int)k};
+    else
+        return {exp2_of(f), (int)k};
+}
+
 // log(1 + e^v). In 32 bits log(u) e / (u - 1) with u = 1 + e^v rounded: the rounding of u cancels.
 __device__ __forceinline__ float softplus(float v) {
     const float e = __builtin_amdgcn_exp2f(v * 1.44269504088896341f), u = 1.0f + e, d = u - 1.0f;
@@ -465,7 +486,8 @@ constexpr int kSegments = 8, kGroup = 8;
 template <typename T>
 __global__ __launch_bounds__(64 * kSegments) void carry_kernel(ScanParams<T> p) {
     constexpr int GROUP = kGroup;
-    __shared__ T left_by[kSegments][64], steps_of[kSegments][64];
+    __shared__ T left_by[kSegments][64];
+    __shared__ LongDecay<T> decay_of[kSegments][64];
     const int seg = threadIdx.y, lane = threadIdx.x, segments = blockDim.y;
     const int64_t own = (int64_t)blockIdx.x * 64 + lane;
     const bool live = own < p.channels;
@@ -477,6 +499,7 @@ __global__ __launch_bounds__(64 * kSegments) void carry_kernel(ScanParams<T> p) 
     for (int c0 = 0; c0 < p.pieces; c0 += segments * GROUP) {
         const int c1 = c0 + seg * GROUP;
         T left[GROUP], steps[GROUP];
+        LongDecay<T> decays[GROUP];
 #pragma unroll
         for (int i = 0; i < GROUP; ++i) {
             const int64_t c = b * p.pieces + c1 + i;
@@ -487,25 +510,26 @@ __global__ __launch_bounds__(64 * kSegments) void carry_kernel(ScanParams<T> p) 
         T h = 0, sum = 0;
 #pragma unroll
         for (int i = 0; i < GROUP; ++i) {
-            h = decay(steps[i], rate) * h + left[i];
+            decays[i] = long_decay(steps[i], rate);
+            h = decays[i](h) + left[i];
             sum += steps[i];
         }
         left_by[seg][lane] = h;
-        steps_of[seg][lane] = sum;
+        decay_of[seg][lane] = long_decay(sum, rate);
         __syncthreads();
         T at = start;
         h = start;
         for (int s = 0; s < segments; ++s) {
             if (s == seg)
                 h = at;
-            at = decay(steps_of[s][lane], rate) * at + left_by[s][lane];
+            at = decay_of[s][lane](at) + left_by[s][lane];
         }
         start = at;
 #pragma unroll
         for (int i = 0; i < GROUP; ++i) {
             if (c1 + i < p.pieces && live)
                 p.carry[((b * p.pieces + c1 + i) * p.states + n) * p.channels + d] = h;
-            h = decay(steps[i], rate) * h + left[i];
+            h = decays[i](h) + left[i];
         }
         __syncthreads(); // the next round writes the shared memory again
     }

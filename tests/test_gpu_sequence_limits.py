@@ -1,0 +1,66 @@
+"""The sequence operators at the limits of what they document: states that grow, prompts in more pieces than one
+round of the carry pass takes, infinite inputs, the precision of the functions they apply, crowds of equal words,
+counts beyond 32 bits."""
+import numpy as np
+import pytest
+
+from tests import sequence_reference as R
+from tests.test_gpu_sequence import close, scan_call, scan_inputs
+
+pytestmark = pytest.mark.gpu
+TYPES = [np.float32, np.float64]
+TOKENS = ("x", "delta", "z", "Bm", "Cm")
+
+
+# ---- the carry pass of a cut scan -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("start", ["zero", "tiny"])
+def test_cut_scan_of_growing_states(dev, dtype, start):
+    """States that grow by more than the type's range over several pieces, from nothing and from a number as
+    small as the type has: the state itself stays in range. Cut, and in parts that are not cut."""
+    B, n, D, N = 1, 700, 64, 16
+    q = scan_inputs(dtype, B, n, D, N, 21)
+    step = 0.7 if dtype == np.float32 else 6.0                # e^95, e^816 over eight pieces of 17 tokens
+    q.update(z=None, skip=None, delta_bias=None)
+    q["delta"][:] = step
+    q["A"][:, ::2], q["A"][:, 1::2] = 1.0, -0.5
+    q["x"][:, :640] = 0
+    if start == "zero":
+        q["state"] = None
+    else:
+        q["state"][:] = 1e-36 if dtype == np.float32 else 1e-300
+        q["delta"][:, 170:] = 0                               # 1e-36 e^119 = 5e15, 1e-300 e^1020 = 1e143
+    y, h, ey, eh = R.state_scan(**q, lengths=None, softplus=False, u=R.half_step(dtype), piece=64)
+    assert np.isfinite(y).all() and np.abs(h).max() > 1e10 and (start == "zero" or np.abs(y[0, 600]).min() > 1e10)
+    got, out, need = scan_call(dev, dtype, q, None, False)
+    assert need > 0
+    close(got, y, ey, "y")
+    # The states that shrink do so by 0.705 or less a token (e^-0.35) until they are below the type's smallest
+    # normal number, where a product loses that number at most: 1 / (1 - 0.705) < 4 of it in all.
+    close(out, h, eh + 4 * float(np.finfo(dtype).tiny), "state")
+    state = q["state"]
+    for at in range(0, n, 90):
+        part = {k: v[:, at:at + 90] if k in TOKENS and v is not None else v for k, v in q.items()}
+        part["state"] = state
+        got, state, need = scan_call(dev, dtype, part, None, False)
+        assert need == 0
+        close(got, y[:, at:at + 90], ey[:, at:at + 90], f"y from token {at}")
+    dev.free_all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,lengths", [(1100, None), (2100, None), (1100, [137]), (2100, [1700])])
+def test_scan_in_more_pieces_than_a_round(dev, dtype, n, lengths):
+    """65 and 124 pieces, where one round of the carry pass takes 64: what a round leaves starts the next, also
+    when the sequence ends in the first round. The state is updated in place."""
+    B, D, N = 1, 64, 16
+    q = scan_inputs(dtype, B, n, D, N, n)
+    q["A"] = (q["A"] / 40).astype(dtype)                      # what the first round leaves is still there in the last
+    y, h, ey, eh = R.state_scan(**q, lengths=lengths, softplus=True, u=R.half_step(dtype), piece=64)
+    got, out, need = scan_call(dev, dtype, q, lengths, True, in_place=True)
+    assert need // (np.dtype(dtype).itemsize * (N + 1) * D) == (65 if n == 1100 else 124)
+    close(got, y, ey, "y")
+    close(out, h, eh, "state")
+    dev.free_all()
