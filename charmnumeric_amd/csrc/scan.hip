@@ -26,6 +26,7 @@
 #include "sequence.h"
 
 #include <algorithm>
+#include <limits>
 #include <type_traits>
 
 using namespace cnh;
@@ -196,16 +197,23 @@ __device__ __forceinline__ int first_state(uint32_t lane) {
     return (int)(lane % S) * (FULL ? NPL : 1);
 }
 
+// Is the lane's i-th state one of the channel's? plan_of() gives a channel more than half of the states that its
+// lanes could hold (one lane of four holds one to four), so only the second half of a lane's can be missing. Those
+// are worked on with the last state's B and C, and kept out of every sum and store whatever becomes of them: a
+// select less than zeros in their place, and an infinite step times input stays out of y.
+template <int NPL, int S, bool FULL>
+__device__ __forceinline__ bool there(int i, int n0, int states) {
+    return FULL || i < (NPL == 4 && S == 1 ? 1 : NPL / 2) || n0 + i * STEP<S, FULL> < states;
+}
+
 // Those of one token's B or C.
 template <typename T, int NPL, int S, bool FULL>
 __device__ __forceinline__ void load_states(T (&v)[NPL], const T* row, int n0, int states) {
     if constexpr (S == 1) {
         Uniform<T>* u = (Uniform<T>*)(uintptr_t)row;
 #pragma unroll
-        for (int i = 0; i < NPL; ++i) {
-            const T at = u[FULL ? i : min(i, states - 1)];
-            v[i] = FULL || i < states ? at : T(0);
-        }
+        for (int i = 0; i < NPL; ++i)
+            v[i] = u[there<NPL, S, FULL>(i, 0, states) ? i : states - 1];
     } else if constexpr (FULL) {
         Pack<T, NPL> q;
         load_pack(q, row + n0);
@@ -213,13 +221,10 @@ __device__ __forceinline__ void load_states(T (&v)[NPL], const T* row, int n0, i
         for (int i = 0; i < NPL; ++i)
             v[i] = q.v[i];
     } else {
-        // the last state again for those that do not exist: no branches between the loads
+        // no branches between the loads
 #pragma unroll
-        for (int i = 0; i < NPL; ++i) {
-            const int n = n0 + i * STEP<S, FULL>;
-            const T at = row[min(n, states - 1)];
-            v[i] = n < states ? at : T(0);
-        }
+        for (int i = 0; i < NPL; ++i)
+            v[i] = row[there<NPL, S, FULL>(i, n0, states) ? n0 + i * STEP<S, FULL> : states - 1];
     }
 }
 
@@ -402,7 +407,7 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
 #pragma unroll
                 for (int i = 0; i < NPL; ++i) {
                     h.v[i] = decay(s[u], rate.v[i]) * h.v[i] + sx * B[i];
-                    sum += C[i] * h.v[i];
+                    sum += there<NPL, S, FULL>(i, n0, p.states) ? C[i] * h.v[i] : T(0);
                 }
                 sum = lanes_sum<S>(sum) + skip * xc[u];
                 if (zp)
@@ -582,7 +587,7 @@ __global__ __launch_bounds__(256) void token_kernel(ScanParams<T> p) {
 #pragma unroll
             for (int i = 0; i < NPL; ++i) {
                 o.h.v[i] = decay(s, rate.v[i]) * o.h.v[i] + sx * o.B[i];
-                out += o.C[i] * o.h.v[i];
+                out += there<NPL, S, FULL>(i, n0, p.states) ? o.C[i] * o.h.v[i] : T(0);
             }
             out = lanes_sum<S>(out) + skip * o.x;
             if (p.z)
@@ -618,6 +623,7 @@ Plan plan_of(const cnh_state_scan_args* a) {
         return s;
     };
     auto waves = [&](int s) { return a->batch * ((D * s + 63) / 64); };
+    // Either way more than half of npl x lanes states exist, or one of four: there() builds on that.
     // Few states per lane spread a small call over more lanes and make a single token's states one
     // 16-byte access each; many states per lane share a token's step and gate. Few as long as the
     // pieces of 32 tokens that the call could be cut into would not fill the device with many.

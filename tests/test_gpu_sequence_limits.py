@@ -1,9 +1,13 @@
 """The sequence operators at the limits of what they document: states that grow, prompts in more pieces than one
 round of the carry pass takes, infinite inputs, the precision of the functions they apply, crowds of equal words,
 counts beyond 32 bits."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
+from charmnumeric_amd import _lib as L
+from tests import helpers as H
 from tests import sequence_reference as R
 from tests.test_gpu_sequence import close, scan_call, scan_inputs
 
@@ -63,4 +67,62 @@ def test_scan_in_more_pieces_than_a_round(dev, dtype, n, lengths):
     assert need // (np.dtype(dtype).itemsize * (N + 1) * D) == (65 if n == 1100 else 124)
     close(got, y, ey, "y")
     close(out, h, eh, "state")
+    dev.free_all()
+
+
+# ---- infinite inputs ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 40, 700])
+@pytest.mark.parametrize("N", [1, 3, 5, 13, 16, 29, 50, 100, 130])
+@pytest.mark.parametrize("skip", [True])
+def test_scan_of_infinite_inputs(dev, dtype, n, N, skip):
+    """An infinite x makes its channel's states and results infinite from there on, and no other's, also where
+    the rows of states are not full."""
+    D, bad, u = 70, n // 2, R.half_step(dtype)
+    q = scan_inputs(dtype, 1, n, D, N, n + N)
+    q["delta"][:] = 0.05
+    q["A"][:] = -np.arange(1, N + 1)
+    for k in ("Bm", "Cm"):
+        q[k] = (np.abs(q[k]) + 0.1).astype(dtype)
+    q.update(z=None, skip=np.abs(q["skip"]) + dtype(0.1) if skip else None, delta_bias=None)
+    y, h, ey, eh = R.state_scan(**q, lengths=None, softplus=False, u=u, piece=64)
+    q["x"][0, bad, 5], q["x"][0, bad, 66] = np.inf, -np.inf
+    got, out, _ = scan_call(dev, dtype, q, None, False)
+    for d, v in ((5, np.inf), (66, -np.inf)):
+        assert (got[0, bad:, d] == v).all() and (out[0, d] == v).all(), (got[0, bad:, d], out[0, d])
+        got[0, bad:, d], out[0, d] = y[0, bad:, d], h[0, d]
+    close(got, y, ey, "y")
+    close(out, h, eh, "state")
+    dev.free_all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [5, 12, 16, 20])
+@pytest.mark.parametrize("skip", [True])
+def test_scan_of_infinite_inputs_in_many_sequences(dev, dtype, N, skip):
+    """The same in batches that fill the device, where a lane has all states of a channel."""
+    B, n, D, bad, u = 1100, 33, 64, 11, R.half_step(dtype)
+    q = scan_inputs(dtype, 1, n, D, N, N)
+    q["delta"][:] = 0.05
+    q["A"][:] = -np.arange(1, N + 1)
+    for k in ("Bm", "Cm"):
+        q[k] = (np.abs(q[k]) + 0.1).astype(dtype)
+    q.update(z=None, skip=np.abs(q["skip"]) + dtype(0.1) if skip else None, delta_bias=None)
+    y, h, ey, eh = R.state_scan(**q, lengths=None, softplus=False, u=u)
+    q["x"][0, bad, 5] = np.inf
+    one, rep = {k: dev.array(v) for k, v in q.items() if v is not None}, dev.array(np.repeat(q["state"], B, axis=0))
+    dy = dev.array(np.full((B, n, D), 7, dtype))
+    a = L.StateScan(H.DT[np.dtype(dtype)], 0, B, n, D, N, one["x"].ptr, 0, D, one["delta"].ptr, 0, D, None, 0, 0, one["A"].ptr,
+                    one["Bm"].ptr, 0, N, one["Cm"].ptr, 0, N, one["skip"].ptr if skip else None, None, rep.ptr, rep.ptr, None, dy.ptr, n * D, D)
+    assert L.lib.cnh_state_scan_workspace(C.byref(a)) == 0
+    L.check(L.lib.cnh_state_scan(C.byref(a), None))
+    got, hs = dy.get(), rep.get()
+    assert (got == got[:1]).all() and (hs == hs[:1]).all()
+    assert (got[0, bad:, 5] == np.inf).all() and (hs[0, 5] == np.inf).all()
+    got, hs = got[:1].copy(), hs[:1].copy()
+    got[0, bad:, 5], hs[0, 5] = y[0, bad:, 5], h[0, 5]
+    close(got, y, ey, "y")
+    close(hs, h, eh, "state")
     dev.free_all()
