@@ -151,6 +151,12 @@ __device__ __forceinline__ T& at(T* row, uint32_t bytes) {
     return *reinterpret_cast<T*>(reinterpret_cast<char*>(row) + bytes);
 }
 
+// v, or 0 (also for what is no number): by a mask in a lane's register, where scalar ones are scarce.
+__device__ __forceinline__ float masked(float v, int32_t mask) { return __int_as_float(__float_as_int(v) & mask); }
+__device__ __forceinline__ double masked(double v, int32_t mask) {
+    return __hiloint2double(__double2hiint(v) & mask, __double2loint(v) & mask);
+}
+
 // v of lane U of every G neighbouring ones (G 2 or 4), in all of them.
 template <int G, int U, typename T>
 __device__ __forceinline__ T from_lane(T v) {
@@ -273,6 +279,8 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
     for (int i = 0; i < NPL; ++i)
         rate.v[i] = rate_of(rate.v[i]);
     const T bias = p.delta_bias ? p.delta_bias[d] : T(0), skip = p.skip ? p.skip[d] : T(0);
+    int32_t keep = p.skip ? -1 : 0; // without a skip nothing of x is added, infinities neither
+    asm("" : "+v"(keep));
 
     const int64_t b = p.first_batch + blockIdx.z;
     const int64_t n = tokens_of(p.lengths, b, p.length);
@@ -409,7 +417,7 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
                     h.v[i] = decay(s[u], rate.v[i]) * h.v[i] + sx * B[i];
                     sum += there<NPL, S, FULL>(i, n0, p.states) ? C[i] * h.v[i] : T(0);
                 }
-                sum = lanes_sum<S>(sum) + skip * xc[u];
+                sum = lanes_sum<S>(sum) + skip * masked(xc[u], keep);
                 if (zp)
                     sum *= gate[u];
                 if (first && live)
@@ -557,6 +565,7 @@ __global__ __launch_bounds__(256) void token_kernel(ScanParams<T> p) {
     for (int i = 0; i < NPL; ++i)
         rate.v[i] = rate_of(rate.v[i]);
     const T bias = p.delta_bias ? p.delta_bias[d] : T(0), skip = p.skip ? p.skip[d] : T(0);
+    const int32_t keep = p.skip ? -1 : 0;
     struct Operands {
         T x, delta, z, B[NPL], C[NPL];
         Pack<T, NPL> h;
@@ -589,7 +598,7 @@ __global__ __launch_bounds__(256) void token_kernel(ScanParams<T> p) {
                 o.h.v[i] = decay(s, rate.v[i]) * o.h.v[i] + sx * o.B[i];
                 out += there<NPL, S, FULL>(i, n0, p.states) ? o.C[i] * o.h.v[i] : T(0);
             }
-            out = lanes_sum<S>(out) + skip * o.x;
+            out = lanes_sum<S>(out) + skip * masked(o.x, keep);
             if (p.z)
                 out *= silu(o.z);
         }

@@ -76,10 +76,10 @@ def test_scan_in_more_pieces_than_a_round(dev, dtype, n, lengths):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n", [1, 40, 700])
 @pytest.mark.parametrize("N", [1, 3, 5, 13, 16, 29, 50, 100, 130])
-@pytest.mark.parametrize("skip", [True])
+@pytest.mark.parametrize("skip", [True, False])
 def test_scan_of_infinite_inputs(dev, dtype, n, N, skip):
     """An infinite x makes its channel's states and results infinite from there on, and no other's, also where
-    the rows of states are not full."""
+    the rows of states are not full and where the call has no skip."""
     D, bad, u = 70, n // 2, R.half_step(dtype)
     q = scan_inputs(dtype, 1, n, D, N, n + N)
     q["delta"][:] = 0.05
@@ -100,7 +100,7 @@ def test_scan_of_infinite_inputs(dev, dtype, n, N, skip):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N", [5, 12, 16, 20])
-@pytest.mark.parametrize("skip", [True])
+@pytest.mark.parametrize("skip", [True, False])
 def test_scan_of_infinite_inputs_in_many_sequences(dev, dtype, N, skip):
     """The same in batches that fill the device, where a lane has all states of a channel."""
     B, n, D, bad, u = 1100, 33, 64, 11, R.half_step(dtype)
