@@ -58,18 +58,27 @@ struct ScanParams {
     T* steps;       // [batch][pieces][channels]: sum of a piece's steps
 };
 
-// exp(s A) with what depends on A alone taken out of the loop: the 32-bit form is one multiplication
-// and the hardware's base-2 exponential (1 ulp); rounding A log2(e) shifts the exponent by at most
-// |s A| 2^-24, which the decay's own size makes harmless. The 64-bit form is the same with a polynomial for
-// the exponential, which wants a finite argument: steps and rates beyond 1e150 are held to it. An infinite
-// rate is held to a finite one in 32 bits too, so that no step (pieces behind a sequence's end) is no decay.
+// exp(s A) with what depends on A alone taken out of the loop. In 32 bits that is one multiplication and the
+// hardware's base-2 exponential (1 ulp); the roundings of A log2(e) and of the product shift the result by |s A| half
+// steps each, which the decay's own size makes harmless. An infinite rate is held to a finite one, so that no step
+// (pieces behind a sequence's end) is no decay.
+// In 64 bits the integer k nearest to t = s rate and the exact s rate - k leave the rounding of A log2(e) alone, |s A|
+// half steps, about what rounding s A costs (110 measured at 100; the rounded t less k 188). Where t is beyond
+// 2^52 the remainder is no small number any more: the polynomial's absolute value, finite as long as steps and
+// rates are held to 1e22, keeps the result at 0 or infinity. The conversion of k saturates, and one instruction
+// more holds the scaling to exponents that it takes (not to the lowest integer).
 __device__ __forceinline__ float rate_of(float a) {
     return a != a ? a : fminf(fmaxf(a * 1.44269504088896341f, -3e38f), 3e38f);
 }
-__device__ __forceinline__ double held(double v) { return fmin(fmax(v, -1e150), 1e150); }
+__device__ __forceinline__ double held(double v) { return fmin(fmax(v, -1e22), 1e22); }
 __device__ __forceinline__ double rate_of(double a) { return a != a ? a : held(a * 1.4426950408889634); }
 __device__ __forceinline__ float decay(float s, float rate) { return __builtin_amdgcn_exp2f(s * rate); }
-__device__ __forceinline__ double decay(double s, double rate) { return exp2_of(held(s) * rate); }
+__device__ __forceinline__ double decay(double s, double rate) {
+    const double v = held(s), k = rint(v * rate);
+    int n; // the instruction itself: a C++ cast says nothing about what does not fit
+    asm("v_cvt_i32_f64 %0, %1" : "=v"(n) : "v"(k));
+    return __builtin_amdgcn_ldexp(fabs(exp2_part(fma(v, rate, -k))), max(min(n, 4096), -4096));
+}
 
 // The decay of many tokens, 2^f 2^k: it can leave the type's range where the state does not (states that grow from
 // nothing or little, or large ones over a long piece). 2^f h scaled by 2^k leaves nothing at nothing, and the range
@@ -89,15 +98,17 @@ __device__ __forceinline__ LongDecay<T> long_decay(T s, T rate) {
     if constexpr (sizeof(T) == 4)
         return {__builtin_amdgcn_exp2f(f), (int)k};
     else
-        return {exp2_of(f), (int)k};
+        return {exp2_part(f), (int)k};
 }
 
-// log(1 + e^v). In 32 bits log(u) e / (u - 1) with u = 1 + e^v rounded: the rounding of u cancels.
+// log(1 + e^v). In 32 bits log(u) e / (u - 1) with u = 1 + e^v rounded (Kahan's log1p): the rounding of u cancels. e^v
+// is the hardware's 2^t for the rounded t = v log2(e), with what the rounding left, v - t log(2), put in.
 __device__ __forceinline__ float softplus(float v) {
-    const float e = __builtin_amdgcn_exp2f(v * 1.44269504088896341f), u = 1.0f + e, d = u - 1.0f;
+    const float a = fmaxf(v, -200.0f), t = a * 1.44269504088896341f, e0 = __builtin_amdgcn_exp2f(t);
+    const float e = fmaf(e0, fmaf(t, -0.693147180559945309f, a), e0), u = 1.0f + e, d = u - 1.0f;
     const float l = __builtin_amdgcn_logf(u) * 0.693147180559945309f;
     const float r = d == 0.0f ? e : l * (e * __builtin_amdgcn_rcpf(d));
-    return v > 20.0f ? v : r;
+    return v <= 20.0f ? r : v; // and what is no number
 }
 // In 64 bits max(v, 0) + log(1 + e) with e = e^-|v|, log(1 + e) = 2 atanh(e / (e + 2)) for small e and
 // log 2 + 2 atanh((e - 1) / (e + 3)) above sqrt(2) - 1, so that the series' argument stays within 0.1716: ten
@@ -493,7 +504,7 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
 // The state each piece starts from, in place of the one it leaves: 64 channels of one state per workgroup,
 // up to kSegments x GROUP pieces a round (as many segments as the pieces need). A lane loads its GROUP
 // pieces at once, folds them to one, takes what the segments before it leave from shared memory and walks
-// its pieces again in registers. 128 pieces of 2048 x 16 fp32 states: 10.7 us; with one lane per channel
+// its pieces again in registers. 128 pieces of 2048 x 16 fp32 states: 11.9 us; with one lane per channel
 // that walks all pieces by itself and waits for memory once per GROUP of them 22.5 us.
 constexpr int kSegments = 8, kGroup = 8;
 template <typename T>

@@ -173,15 +173,10 @@ __device__ __forceinline__ int64_t tokens_of(const int32_t* lengths, int64_t b, 
     return n < 0 ? 0 : n < length ? n : length;
 }
 
-// 2^t for finite t, to an ulp: 2^k times a polynomial in t - k for the nearest integer k, the interpolation of
-// 2^f at the Chebyshev nodes of [-1/2, 1/2] (2^-55 off at most, its rounded coefficients included). The
-// library's exponential spends a third of its instructions on its range; here the conversion of k saturates,
-// and one instruction more holds the scaling to exponents that it takes (not to the lowest integer).
-__device__ __forceinline__ double exp2_of(double t) {
-// t - k without the product behind t drawn into it: its rounding error is no part of f, and would be far from
-// small where t is large.
-#pragma clang fp contract(off)
-    const double k = rint(t), f = t - k;
+// 2^f for |f| <= 1/2 and a little more: the interpolation of 2^f at the Chebyshev nodes of [-1/2, 1/2] by a polynomial
+// (2^-55 off at most, its rounded coefficients included). The library's exponential spends a third of its
+// instructions on its range.
+__device__ __forceinline__ double exp2_part(double f) {
     double p = 4.4558179083360645e-10;
     p = fma(p, f, 7.074194297288521e-09);
     p = fma(p, f, 1.0178057087733941e-07);
@@ -193,19 +188,25 @@ __device__ __forceinline__ double exp2_of(double t) {
     p = fma(p, f, 0.055504108664821625);
     p = fma(p, f, 0.24022650695910158);
     p = fma(p, f, 0.6931471805599453);
-    p = fma(p, f, 1.0);
-    int n; // the instruction itself: a C++ cast says nothing about what does not fit
-    asm("v_cvt_i32_f64 %0, %1" : "=v"(n) : "v"(k));
-    return __builtin_amdgcn_ldexp(p, max(min(n, 4096), -4096));
+    return fma(p, f, 1.0);
 }
-// e^-|x|; 0 for NaN.
+// e^-|x| to 0.75 ulp: 2^(t - k) 2^k for t = -|x| log2(e), k the integer nearest to it. t - k is formed from the
+// exact product with log2(e) in two parts: the rounded t alone would be off by |x| half steps (x = -20: 14 measured,
+// 1.5 so). 0 for NaN.
 __device__ __forceinline__ double exp_of_minus(double x) {
-    return exp2_of(fmax(fabs(x) * -1.4426950408889634, -2000.0));
+    const double a = fmin(fabs(x), 2000.0), k = rint(a * -1.4426950408889634);
+    const double f = fma(a, -2.0355273740931033e-17, fma(a, -1.4426950408889634, -k));
+    return __builtin_amdgcn_ldexp(exp2_part(f), (int)k);
 }
 
-// x * sigmoid(x)
+// x * sigmoid(x). In 32 bits e^-x is the hardware's 2^t for the rounded t = -x log2(e), with what the rounding left,
+// r = -x - t log(2), put in; without it the result is off by |x| half steps (18 on [-20, -10]). t is held to what 2^t can
+// be: r makes up for it where x is below -87, until the reciprocal is 0 (results of 2^-120 and less; it has no
+// denormals). The maximum is for 0 times infinity, at x = infinity.
 __device__ __forceinline__ float silu(float x) {
-    return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f));
+    const float t = __builtin_amdgcn_fmed3f(x * -1.44269504088896341f, -150.0f, 126.0f);
+    const float e = __builtin_amdgcn_exp2f(t), r = fmaf(t, -0.693147180559945309f, -x);
+    return x * __builtin_amdgcn_rcpf(fmaxf(1.0f + fmaf(e, r, e), 1.0f));
 }
 __device__ __forceinline__ double silu(double x) {
     const double e = exp_of_minus(x);

@@ -9,7 +9,7 @@ import pytest
 from charmnumeric_amd import _lib as L
 from tests import helpers as H
 from tests import sequence_reference as R
-from tests.test_gpu_sequence import close, scan_call, scan_inputs
+from tests.test_gpu_sequence import close, conv_call, scan_call, scan_inputs
 
 pytestmark = pytest.mark.gpu
 TYPES = [np.float32, np.float64]
@@ -125,4 +125,86 @@ def test_scan_of_infinite_inputs_in_many_sequences(dev, dtype, N, skip):
     got[0, bad:, 5], hs[0, 5] = y[0, bad:, 5], h[0, 5]
     close(got, y, ey, "y")
     close(hs, h, eh, "state")
+    dev.free_all()
+
+
+# ---- the functions' own precision -----------------------------------------------------------------
+
+
+def spread(dtype, far, seed, n=40000):
+    """Numbers of every size up to `far`, of both signs."""
+    rng = np.random.default_rng(seed)
+    v = np.concatenate([rng.uniform(-far, far, n), rng.uniform(-20, 20, n), np.exp(rng.uniform(-9, 0, n)) * rng.choice([-1, 1], n)])
+    return v.astype(dtype)
+
+
+def within(got, want, half_steps, v, dtype, what):
+    """got is off from want by so many half steps of the type at most (relative to want)."""
+    e = np.abs((got.astype(np.longdouble) - want) / want) / R.half_step(dtype)
+    over = ~(e <= half_steps)
+    assert not over.any(), (what, int(over.sum()), float(e[over].max()), v[over][:4], e[over][:4].astype(float))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_precision_of_the_activation(dev, dtype):
+    """v sigmoid(v), through a convolution of one tap. e^-v to within 2.2 half steps in 64 bits (its remainder
+    0.35, its polynomial 0.25 and 1.5), 1 + e^-v, quotient and product 1 each. In 32 bits the hardware's exponential
+    (an ulp, 2 half steps; log 2 in 24 bits 0.046 |v|), what its argument's rounding left, 1 + e^-v and the product 1
+    each, the reciprocal 2."""
+    v = spread(dtype, 80 if dtype == np.float32 else 690, 1)
+    v = v[v != 0]
+    got, _ = conv_call(dev, dtype, v.reshape(1, 1, -1), np.ones((1, v.size), dtype), None, None, None, True)
+    x = v.astype(np.longdouble)
+    within(got.reshape(-1), x / (1 + np.exp(-x)), 7.5 + 0.05 * np.abs(v) if dtype == np.float32 else 6.0, v, dtype, "silu")
+    ends = np.array([0.0, -0.0, np.inf, -1e30, 1e30, np.nan, -1000], dtype)
+    got, _ = conv_call(dev, dtype, ends.reshape(1, 1, -1), np.ones((1, ends.size), dtype), None, None, None, True)
+    assert np.array_equal(got.reshape(-1), np.array([0, 0, np.inf, 0, 1e30, np.nan, 0], dtype), equal_nan=True)
+    dev.free_all()
+
+
+def one_token(dtype, D, **kw):
+    """A scan of one token and one state per channel: y = exp(s A) h + s."""
+    q = dict(x=np.ones((1, 1, D), dtype), delta=np.zeros((1, 1, D), dtype), z=None, A=np.zeros((D, 1), dtype),
+             Bm=np.ones((1, 1, 1), dtype), Cm=np.ones((1, 1, 1), dtype), skip=None, delta_bias=None, state=None)
+    q.update(kw)
+    return q
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_precision_of_the_step(dev, dtype):
+    """log(1 + e^v). 64 bits: e^-|v| 2.2 half steps, denominator, quotient and its last product 1 each, the sum 1.
+    32 bits: exponential 2 (and 0.046 |v|), logarithm 2 and a product, reciprocal 2 and two products, and what of the
+    rounding of 1 + e^v does not cancel, 1."""
+    v = spread(dtype, 80 if dtype == np.float32 else 690, 2)
+    y, _, _ = scan_call(dev, dtype, one_token(dtype, v.size, delta=v.reshape(1, 1, -1)), None, True)
+    x = v.astype(np.longdouble)
+    within(y.reshape(-1), np.log1p(np.exp(-np.abs(x))) + np.maximum(x, 0), 10 + 0.05 * np.abs(v) if dtype == np.float32 else 6.2, v,
+           dtype, "softplus")
+    ends = np.array([-np.inf, np.inf, np.nan, -1e30, 1e30, 0], dtype)
+    y, _, _ = scan_call(dev, dtype, one_token(dtype, ends.size, delta=ends.reshape(1, 1, -1), x=np.ones((1, 1, ends.size), dtype)),
+                        None, True)
+    assert np.array_equal(y.reshape(-1)[[0, 3, 4]], np.array([0, 0, 1e30], dtype)) and np.isnan(y.reshape(-1)[2])
+    assert abs(y.reshape(-1)[5] - np.log(2)) < 4 * R.half_step(dtype)
+    dev.free_all()
+
+
+def test_precision_of_the_decay(dev):
+    """exp(s A) in 64 bits: one rounding of A log2(e) (and 0.13 of its constant's), each |s A| half steps, and the
+    exponential's 2.2. What e^(s A) of a single state loses by rounding s A alone is |s A|."""
+    rng = np.random.default_rng(3)
+    n = 60000
+    s = np.exp(rng.uniform(-8, 3, n))
+    A = -rng.uniform(0, 100, n) / s
+    A[:n // 8] *= -1
+    zero = np.zeros((1, 1, n))
+    y, _, _ = scan_call(dev, np.float64, one_token(np.float64, n, x=zero, delta=s.reshape(1, 1, -1), A=A.reshape(-1, 1),
+                                                   state=np.ones((1, n, 1))), None, False)
+    t = s.astype(np.longdouble) * A.astype(np.longdouble)
+    within(y.reshape(-1), np.exp(t), 1.2 * np.abs(s * A) + 3.2, s * A, np.float64, "decay")
+    # far arguments on both sides, and none
+    s = np.array([1e21, 1e21, 1.0, 0.0, 3.0, 1e10, 1e10])
+    A = np.array([-1e21, 1e21, -1e5, -np.inf, -np.inf, 1e10, -1e10])
+    y, _, _ = scan_call(dev, np.float64, one_token(np.float64, 7, x=np.zeros((1, 1, 7)), delta=s.reshape(1, 1, -1),
+                                                   A=A.reshape(-1, 1), state=np.ones((1, 7, 1))), None, False)
+    assert y.reshape(-1).tolist() == [0, np.inf, 0, 1, 0, np.inf, 0]
     dev.free_all()
