@@ -16,6 +16,7 @@
 #include "sequence.h"
 
 #include <algorithm>
+#include <limits>
 
 using namespace cnh;
 
@@ -217,7 +218,8 @@ int run(const cnh_rms_norm_args* a, hipStream_t st) {
     p.residual_out = static_cast<T*>(a->residual_out);
     p.residual_out_stride = a->residual_out_stride;
     p.weight = static_cast<const T*>(a->weight);
-    p.eps = (T)a->eps;
+    // an eps below the type's smallest number counts as that: it keeps a row of zeros one
+    p.eps = a->eps > 0 ? std::max((T)a->eps, std::numeric_limits<T>::denorm_min()) : T(0);
     p.y = static_cast<T*>(a->y);
     p.y_stride = a->y_stride;
     constexpr int W = Wide<T>::n;

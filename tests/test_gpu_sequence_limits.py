@@ -208,3 +208,20 @@ def test_precision_of_the_decay(dev):
                                                    A=A.reshape(-1, 1), state=np.ones((1, 7, 1))), None, False)
     assert y.reshape(-1).tolist() == [0, np.inf, 0, 1, 0, np.inf, 0]
     dev.free_all()
+
+
+# ---- the norm's eps -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,eps", [(np.float32, 1e-50), (np.float32, 1e-45), (np.float32, 1e-39), (np.float64, 5e-324)])
+def test_norm_of_zeros_with_an_eps_below_the_type(dev, dtype, eps):
+    """An eps that is not zero keeps a row of zeros one, however small it is."""
+    for cols in (40, 41, 9000):
+        x = np.zeros((2, cols), dtype)
+        x[1] = 1
+        dx, dy = dev.array(x), dev.array(np.full_like(x, 3))
+        a = L.RmsNorm(H.DT[np.dtype(dtype)], 2, cols, dx.ptr, cols, None, 0, None, 0, None, eps, dy.ptr, cols)
+        L.check(L.lib.cnh_rms_norm(C.byref(a), None))
+        got = dy.get()
+        assert (got[0] == 0).all() and np.abs(got[1] - 1).max() <= 8 * R.half_step(dtype)
+    dev.free_all()
