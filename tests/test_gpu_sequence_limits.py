@@ -9,7 +9,7 @@ import pytest
 from charmnumeric_amd import _lib as L
 from tests import helpers as H
 from tests import sequence_reference as R
-from tests.test_gpu_sequence import close, conv_call, scan_call, scan_inputs
+from tests.test_gpu_sequence import close, conv_call, sample_call, scan_call, scan_inputs
 
 pytestmark = pytest.mark.gpu
 TYPES = [np.float32, np.float64]
@@ -224,4 +224,46 @@ def test_norm_of_zeros_with_an_eps_below_the_type(dev, dtype, eps):
         L.check(L.lib.cnh_rms_norm(C.byref(a), None))
         got = dy.get()
         assert (got[0] == 0).all() and np.abs(got[1] - 1).max() <= 8 * R.half_step(dtype)
+    dev.free_all()
+
+
+# ---- crowds of equal words ------------------------------------------------------------------------
+
+
+def crowds(dtype):
+    rng = np.random.default_rng(3)
+    V = 20000
+    rows = [np.zeros(V), rng.integers(0, 3, V), 1 + 1e-4 * rng.random(V), np.where(rng.random(V) < 0.5, 0.0, -0.0),
+            np.repeat([5.0, 4.999, -3.0, 5.0], V // 4), 1e-3 * rng.integers(0, 5000, V) / 5000 + 4]
+    return np.stack(rows).astype(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("top_k,top_p,min_p", [(700, 0.50031, 0.0), (5000, 0.90017, 0.0), (0, 0.30013, 0.5), (12001, 0.77777, 0.2),
+                                               (300, 0.50113, 0.0), (19999, 0.99987, 0.0)])
+def test_sample_crowds_cut_between_words(dev, dtype, top_k, top_p, min_p):
+    """Cuts that fall clearly between two words of a crowd, and draws that do: every row is checked."""
+    logits = crowds(dtype)
+    u = np.array([0.31417, 0.62713, 0.50123, 0.87117, 0.99991, 0.01237])
+    want = [R.sample_tokens(logits[r], u[r], 1.0, top_k, top_p, min_p) for r in range(len(u))]
+    assert min(near for _, near in want) > logits.shape[1] * 2.0 ** -45
+    got = sample_call(dev, logits, u, 1.0, top_k, top_p, min_p)
+    assert got.tolist() == [w for w, _ in want]
+    for r in range(len(u)):                                   # few rows are weighed in slices, one by one too
+        assert sample_call(dev, logits[r:r + 1], u[r:r + 1], 1.0, top_k, top_p, min_p)[0] == got[r]
+    dev.free_all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("top_k,top_p", [(700, 0.5), (5000, 0.9), (0, 0.3), (300, 0.25)])
+def test_sample_crowds_cut_at_a_word(dev, dtype, top_k, top_p):
+    """Rows of one value where top_p of top_k is a whole number of words: the cut is at that word or, as
+    the product rounds, the one after it, and the word drawn follows from the cut."""
+    V = 20000
+    u = np.array([0.0, 0.31417, 0.62713, 0.87117, 0.99991])
+    logits = np.repeat(np.array([[0.0], [-7.5], [3.0], [np.finfo(dtype).min], [1.0]]), V, axis=1).astype(dtype)
+    whole = round(top_p * (top_k or V))
+    got = sample_call(dev, logits, u, 1.0, top_k, top_p)
+    for r in range(len(u)):
+        assert got[r] in {int(u[r] * whole), int(u[r] * (whole + 1))}, (r, got[r], whole)
     dev.free_all()
