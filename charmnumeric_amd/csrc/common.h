@@ -73,6 +73,9 @@ void gemm_set_ksplit(int on);
 int gemm_form(int64_t M, int64_t N, int64_t K, const void* A, int64_t lda, const void* B, int64_t ldb);
 int reduce_slots_f64(bool maximum, double* slots, int64_t n, double* out, hipStream_t st);
 
+// out[i] = in[i] held to 32 bits, on the stream.
+int narrow_counts(const int64_t* in, int32_t* out, int64_t n, hipStream_t st);
+
 // Option "product_statements": may a product's launch evaluate the statements that follow it?
 bool product_statements_on();
 

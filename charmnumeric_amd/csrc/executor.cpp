@@ -4747,6 +4747,42 @@ int seq_whole(Ex* ex, const char* call, const char* what, int name, int dtype, i
     return 0;
 }
 
+// Integers, one per sequence or row: int32 as they are, int64 held to 32 bits in a buffer that goes back to the free
+// list with the object (what takes it next runs behind the call on the stream).
+struct SeqCounts {
+    Ex* ex = nullptr;
+    size_t bytes = 0;
+    void* buffer = nullptr;
+    const int32_t* ptr = nullptr;
+    ~SeqCounts() {
+        if (buffer)
+            slab_release(ex, bytes, buffer);
+    }
+};
+int seq_counts(Ex* ex, const char* call, const char* what, int name, int64_t n, SeqCounts* out) {
+    if (name == 0)
+        return 0;
+    XArray* a;
+    if (int rc = find_array(ex, name, &a, call))
+        return rc;
+    const bool wide = a->dtype == CNH_I64;
+    void* p;
+    if (int rc = seq_whole(ex, call, what, name, wide ? CNH_I64 : CNH_I32, 1, &n, &p))
+        return rc;
+    if (!wide) {
+        out->ptr = static_cast<const int32_t*>(p);
+        return 0;
+    }
+    out->ex = ex;
+    out->bytes = ((size_t)n * 4 + 255) & ~(size_t)255;
+    if (int rc = slab_alloc(ex, out->bytes, false, &out->buffer))
+        return rc;
+    out->ptr = static_cast<const int32_t*>(out->buffer);
+    if (ex->trace_on) ex->log("narrow " + std::to_string(name) + " for " + call);
+    return ex->dry ? 0 : narrow_counts(static_cast<const int64_t*>(p), static_cast<int32_t*>(out->buffer), n,
+                                       as_stream(ex->stream));
+}
+
 // batch x length x columns: rank 3, or rank 2 as one token per sequence.
 struct SeqRows {
     int64_t batch = 0, length = 0, cols = 0, batch_stride = 0, stride = 0;
@@ -4858,17 +4894,18 @@ int cnx_short_convolution(cnx_executor* ex, const cnx_short_convolution_args* q)
     a.batch = x.batch, a.length = x.length, a.channels = x.cols;
     a.x = x.ptr, a.x_batch_stride = x.batch_stride, a.x_stride = x.stride;
     const int64_t wext[2] = {a.taps, a.channels}, sext[3] = {a.batch, a.taps - 1, a.channels};
-    void *weight, *bias, *state, *lengths;
+    void *weight, *bias, *state;
+    SeqCounts lengths;
     if (int rc = seq_whole(ex, call, "weight", q->weight, dtype, 2, wext, &weight))
         return rc;
     if (int rc = seq_whole(ex, call, "bias", q->bias, dtype, 1, wext + 1, &bias))
         return rc;
     if (int rc = seq_whole(ex, call, "state", q->state, dtype, 3, sext, &state))
         return rc;
-    if (int rc = seq_whole(ex, call, "lengths", q->lengths, CNH_I32, 1, &a.batch, &lengths))
+    if (int rc = seq_counts(ex, call, "lengths", q->lengths, a.batch, &lengths))
         return rc;
     a.weight = weight, a.bias = bias, a.state_in = a.state_out = state;
-    a.lengths = static_cast<const int32_t*>(lengths);
+    a.lengths = lengths.ptr;
     const int64_t ext3[3] = {a.batch, a.length, a.channels}, ext2[2] = {a.batch, a.channels};
     XArray* y;
     if (int rc = seq_result(ex, q->y, nd, dtype, nd == 3 ? ext3 : ext2, &y))
@@ -4908,7 +4945,8 @@ int cnx_state_scan(cnx_executor* ex, const cnx_state_scan_args* q) {
     a.B = B.ptr, a.B_batch_stride = B.batch_stride, a.B_stride = B.stride;
     a.C = C.ptr, a.C_batch_stride = C.batch_stride, a.C_stride = C.stride;
     const int64_t aext[2] = {a.channels, a.states}, sext[3] = {a.batch, a.channels, a.states};
-    void *A, *skip, *bias, *state, *lengths;
+    void *A, *skip, *bias, *state;
+    SeqCounts lengths;
     CNH_CHECK(q->A != 0, -2, "%s: no A", call);
     if (int rc = seq_whole(ex, call, "A", q->A, dtype, 2, aext, &A))
         return rc;
@@ -4918,10 +4956,10 @@ int cnx_state_scan(cnx_executor* ex, const cnx_state_scan_args* q) {
         return rc;
     if (int rc = seq_whole(ex, call, "state", q->state, dtype, 3, sext, &state))
         return rc;
-    if (int rc = seq_whole(ex, call, "lengths", q->lengths, CNH_I32, 1, &a.batch, &lengths))
+    if (int rc = seq_counts(ex, call, "lengths", q->lengths, a.batch, &lengths))
         return rc;
     a.A = A, a.skip = skip, a.delta_bias = bias, a.state_in = a.state_out = state;
-    a.lengths = static_cast<const int32_t*>(lengths);
+    a.lengths = lengths.ptr;
     const int64_t need = cnh_state_scan_workspace(&a);
     if (need < 0)
         return (int)need;
@@ -4966,12 +5004,13 @@ int cnx_sample_tokens(cnx_executor* ex, const cnx_sample_tokens_args* q) {
     a.top_k = q->top_k;
     a.temperature = q->temperature, a.top_p = q->top_p, a.min_p = q->min_p;
     CNH_CHECK(q->u != 0, -2, "%s: no random numbers", call);
-    void *u, *t, *k, *p, *m;
+    void *u, *t, *p, *m;
+    SeqCounts k;
     if (int rc = seq_whole(ex, call, "u", q->u, CNH_F64, 1, &a.rows, &u))
         return rc;
     if (int rc = seq_whole(ex, call, "temperature", q->temperatures, CNH_F64, 1, &a.rows, &t))
         return rc;
-    if (int rc = seq_whole(ex, call, "top_k", q->top_ks, CNH_I32, 1, &a.rows, &k))
+    if (int rc = seq_counts(ex, call, "top_k", q->top_ks, a.rows, &k))
         return rc;
     if (int rc = seq_whole(ex, call, "top_p", q->top_ps, CNH_F64, 1, &a.rows, &p))
         return rc;
@@ -4979,7 +5018,7 @@ int cnx_sample_tokens(cnx_executor* ex, const cnx_sample_tokens_args* q) {
         return rc;
     a.u = static_cast<const double*>(u);
     a.temperatures = static_cast<const double*>(t);
-    a.top_ks = static_cast<const int32_t*>(k);
+    a.top_ks = k.ptr;
     a.top_ps = static_cast<const double*>(p);
     a.min_ps = static_cast<const double*>(m);
     const int64_t need = cnh_sample_tokens_workspace(&a);

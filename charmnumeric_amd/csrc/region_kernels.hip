@@ -97,6 +97,12 @@ int launch_convert(int dst_dtype, void* dst, const void* src, const RegionArgs& 
     return 0;
 }
 
+__global__ __launch_bounds__(kBlock) void narrow_kernel(const int64_t* __restrict__ in, int32_t* __restrict__ out, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (i < n)
+        out[i] = (int32_t)(in[i] < INT32_MIN ? INT32_MIN : in[i] > INT32_MAX ? INT32_MAX : in[i]);
+}
+
 __global__ __launch_bounds__(256) void zero_kernel(uint4* __restrict__ p, size_t n16,
                                                    unsigned char* __restrict__ tail_base,
                                                    size_t tail) {
@@ -134,6 +140,14 @@ int pack_args(int nd, const int64_t* dstr, const int64_t* dsta, const int64_t* d
 }
 
 } // namespace
+
+int cnh::narrow_counts(const int64_t* in, int32_t* out, int64_t n, hipStream_t st) {
+    if (n < 1)
+        return 0;
+    hipLaunchKernelGGL(narrow_kernel, dim3((unsigned)((n + kBlock - 1) / kBlock)), dim3(kBlock), 0, st, in, out, n);
+    CNH_HIP(hipGetLastError());
+    return 0;
+}
 
 extern "C" {
 

@@ -71,13 +71,24 @@ def _whole(x, what, shape, dtype):
     return x.copy() if isinstance(x, ArrayView) and not _is_whole(x.region, x.base.shape) else x
 
 
-def _lengths(x, batch):
-    if x is None:
-        return None
-    x = asarray(x) if isinstance(x, _ArrayLike) else asarray(np.asarray(x, dtype=_I32))
+def _counts(x, what, n):
+    """Integers, one per sequence or row: held to 32 bits, here where they are the host's, by the executor
+    where they are an Array of 64 bits."""
+    if not isinstance(x, _ArrayLike):
+        x = np.asarray(x)
+        if x.dtype.kind in "iu":
+            here, to = np.iinfo(x.dtype), np.iinfo(_I32)
+            x = np.clip(x, max(here.min, to.min), min(here.max, to.max))
+        elif x.dtype.kind != "b":
+            raise TypeError(f"{what} must be integers, got {x.dtype.name}")
+        x = asarray(x.astype(_I32))
     if x.dtype.kind != "i":
-        raise TypeError(f"lengths must be integers, got {x.dtype.name}")
-    return _whole(x, "lengths", (batch,), _I32)
+        raise TypeError(f"{what} must be integers, got {x.dtype.name}")
+    return _whole(x, what, (n,), x.dtype)
+
+
+def _lengths(x, batch):
+    return None if x is None else _counts(x, "lengths", batch)
 
 
 def _sliced(x, even_rows=False):
@@ -144,7 +155,8 @@ def short_convolution(x, weight, bias=None, state=None, lengths=None, activation
 
     state, (batch, taps - 1, channels): the rows in front of the first token (None: zeros), which become
     the last rows of each sequence, so that the next call goes on where this one ended. lengths: how many
-    of the `length` tokens each sequence has (None: all); rows of the result behind them are zeros."""
+    of the `length` tokens each sequence has, integers of any width (None: all); rows of the result behind
+    them are zeros."""
     x, weight, bias = _operand(x, "x"), _operand(weight, "weight"), _operand(bias, "bias")
     lead = _rows_of(x, "x", "short_convolution")
     if activation not in ("silu", None):
@@ -204,10 +216,7 @@ def state_scan(x, delta, A, B, C, skip=None, z=None, delta_bias=None, state=None
 def _setting(v, what, rows, dtype, lowest, highest):
     """(scalar, array or None) of a setting that is either one number or one per row."""
     if not _is_scalar_like(v):
-        v = _operand(v, what)
-        if dtype == _I32 and v.dtype.kind != "i":
-            raise TypeError(f"{what} must be integers, got {v.dtype.name}")
-        return 0, _whole(v, what, (rows,), dtype)
+        return 0, _counts(v, what, rows) if dtype == _I32 else _whole(_operand(v, what), what, (rows,), dtype)
     v = _coerce_scalar(v)
     if dtype == _I32 and not isinstance(v, int):
         raise TypeError(f"{what} must be an integer, got {v!r}")

@@ -188,7 +188,8 @@ typedef struct cnx_rms_norm_args {
 } cnx_rms_norm_args;
 int cnx_rms_norm(cnx_executor* ex, const cnx_rms_norm_args* args);
 /* x (batch, length, channels), or (batch, channels) for one token per sequence; weight (taps, channels),
- * bias (channels), state (batch, taps - 1, channels; updated), lengths int32 (batch). */
+ * bias (channels), state (batch, taps - 1, channels; updated), lengths int32 or int64 (batch; int64 is held to
+ * 32 bits). */
 typedef struct cnx_short_convolution_args {
     cnx_operand x;
     int32_t weight, bias, state, lengths, y;
@@ -196,7 +197,7 @@ typedef struct cnx_short_convolution_args {
 } cnx_short_convolution_args;
 int cnx_short_convolution(cnx_executor* ex, const cnx_short_convolution_args* args);
 /* x, delta, z like the convolution's x; B, C (batch, length, states) or (batch, states); A (channels,
- * states), skip and delta_bias (channels), state (batch, channels, states; updated), lengths int32 (batch). */
+ * states), skip and delta_bias (channels), state (batch, channels, states; updated), lengths as above. */
 typedef struct cnx_state_scan_args {
     cnx_operand x, delta, z, B, C;
     int32_t A, skip, delta_bias, state, lengths, y;
@@ -204,7 +205,7 @@ typedef struct cnx_state_scan_args {
 } cnx_state_scan_args;
 int cnx_state_scan(cnx_executor* ex, const cnx_state_scan_args* args);
 /* logits (rows, vocab) or (vocab); u fp64 (rows); temperatures, top_ps, min_ps fp64 (rows) and top_ks
- * int32 (rows) where not 0 instead of the scalars; out: int32 (rows). */
+ * int32 or int64 (rows; int64 is held to 32 bits) where not 0 instead of the scalars; out: int32 (rows). */
 typedef struct cnx_sample_tokens_args {
     cnx_operand logits;
     int32_t u, temperatures, top_ks, top_ps, min_ps, out;

@@ -6,6 +6,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
+import charmnumeric_amd as cnp
 from charmnumeric_amd import _lib as L
 from tests import helpers as H
 from tests import sequence_reference as R
@@ -267,3 +268,53 @@ def test_sample_crowds_cut_at_a_word(dev, dtype, top_k, top_p):
     for r in range(len(u)):
         assert got[r] in {int(u[r] * whole), int(u[r] * (whole + 1))}, (r, got[r], whole)
     dev.free_all()
+
+
+# ---- counts beyond 32 bits ------------------------------------------------------------------------
+
+
+@pytest.fixture(params=["plain", "tiles", "pipeline"])
+def itf(request):
+    cnp.reset()
+    it = cnp.CharmNumericInterface(device=0)
+    it.connect(odf=64 if request.param == "tiles" else 4)
+    if request.param == "tiles":
+        it.set_min_tile(1, 2)
+    if request.param == "pipeline":
+        it.set_pipeline()
+    yield it
+    cnp.reset()
+    it.close()
+
+
+@pytest.mark.parametrize("where", ["host", "array", "slice"])
+def test_counts_of_64_bits_are_held_to_their_range(itf, where):
+    """lengths and top_k of 64-bit integers mean what they say: beyond the sequence all of it, negative none."""
+    rng = np.random.default_rng(6)
+
+    def given(values):
+        v = np.array(values, np.int64)
+        if where == "host":
+            return v
+        if where == "array":
+            return cnp.array(v)
+        return cnp.array(np.concatenate([[7], v, [9]]))[1:-1]
+
+    x, w = rng.standard_normal((5, 9, 8)), rng.standard_normal((3, 8))
+    lengths = [2 ** 32 + 3, -2 ** 40, 4, 2 ** 31, -2 ** 32 + 2]
+    y, _, ey = R.short_convolution(x, w, None, None, [9, 0, 4, 9, 0], True, R.half_step(np.float64))
+    got = cnp.short_convolution(cnp.array(x), cnp.array(w), lengths=given(lengths)).get(itf)
+    close(got, y, ey, "convolution")
+    q = scan_inputs(np.float64, 5, 9, 8, 4, 1)
+    a = {k: cnp.array(v) for k, v in q.items()}
+    y, h, ey, eh = R.state_scan(**q, lengths=[9, 0, 4, 9, 0], softplus=True, u=R.half_step(np.float64))
+    got = cnp.state_scan(a["x"], a["delta"], a["A"], a["Bm"], a["Cm"], a["skip"], a["z"], a["delta_bias"], a["state"],
+                         given(lengths))
+    close(got.get(itf), y, ey, "scan")
+    close(a["state"].get(itf), h, eh, "state")
+
+    logits, u = 2 * rng.standard_normal((5, 300)), rng.random(5)
+    ks = [2 ** 32 + 1, 2 ** 31 + 3, 5, -2 ** 32 + 1, 2 ** 33]
+    got = cnp.random.sample_tokens(cnp.array(logits), u, 1.0, given(ks)).get(itf)
+    want = [R.sample_tokens(logits[r], u[r], 1.0, k, 1.0, 0.0)[0] for r, k in enumerate([0, 0, 5, 0, 0])]
+    assert got.tolist() == want
