@@ -647,15 +647,16 @@ Plan plan_of(const cnh_state_scan_args* a) {
     // Few states per lane spread a small call over more lanes and make a single token's states one
     // 16-byte access each; many states per lane share a token's step and gate. Few as long as the
     // pieces of 32 tokens that the call could be cut into would not fill the device with many.
-    // For 33 to 64 states few are faster always (64 states, 2048 channels, sixteen a lane and four: 16 x 100
-    // tokens 116 and 97 us in fp32, 397 and 311 in fp64; 4 x 300 tokens 139 and 102, 478 and 242).
-    // A lane whose many are not all there reads B and C element by element: in uncut calls few are faster
-    // with less than a wavefront per unit (22 x 200 tokens of 2048 channels, 12 states: 223 and 113 us in fp32,
-    // 485 and 350 in fp64; 62 x 200 tokens, 10 states: 259 and 292, 592 and 909), and from 17 states on always
-    // (65 x 100 tokens, 20 states: 354 and 282, 1022 and 924).
+    // For 33 to 64 states few are taken always (64 states, 2048 channels, sixteen a lane and four: 16 x 100
+    // tokens 109 and 110 us in fp32, 384 and 300 in fp64; 4 x 300 tokens 133 and 103, 472 and 224; with 50 states
+    // 16 x 100 tokens would take 88 instead of 122, 249 instead of 343).
+    // Where a lane's many are not all there, few are faster in uncut calls with less than a wavefront per unit
+    // (many and few, 22 x 200 tokens of 2048 channels, 12 states: 172 and 103 us in fp32, 344 and 302 in fp64; 23 x 100,
+    // 20 states: 126 and 93, 319 and 269), many beyond (62 x 200 tokens, 10 states: 193 and 265, 471 and 734;
+    // 65 x 100, 20 states: 204 and 264, 682 and 714; 130 x 50, 31 states: 206 and 275, 628 and 733).
     const int many = N <= 8 || (N > 64 && N <= 128) ? 8 : N <= 16 || N > 128 ? 16 : 32;
     const int64_t wm = waves(lanes(many));
-    const bool sparse = N != many && wm > kUnits * 5 / 8 && (N > 16 || wm < kUnits);
+    const bool sparse = N != many && wm > kUnits * 5 / 8 && wm < kUnits;
     q.npl = many;
     if (N <= 64 && (N > 32 || N <= 4 || L <= 1 || wm * std::max<int64_t>(1, L / 32) < 2 * kUnits || sparse))
         q.npl = 4;
@@ -668,11 +669,11 @@ Plan plan_of(const cnh_state_scan_args* a) {
         q.piece = std::max<int64_t>(1, (a->batch + slices - 1) / slices);
         q.piece = std::max(q.piece, (a->batch + 65534) / 65535);
     } else {
-        // Measured with 300 tokens of 2048 fp32 channels, 16 states: 16 sequences (512 wavefronts) 120 us
-        // uncut, 95 us in 8 pieces; 24 sequences (768) 129 us uncut, 134 us in 3. With 256 channels of
-        // 2 sequences: 64 tokens 20 us uncut, 22 us in 4 pieces; 128 tokens 29 and 22 us. Where B and C do
+        // Measured with 300 tokens of 2048 fp32 channels, 16 states: 16 sequences (512 wavefronts) 126 us
+        // uncut, 101 us in 8 pieces; 24 sequences (768) 134 us uncut, 140 us in 3. With 256 channels of
+        // 2 sequences: 64 tokens 17 us uncut, 23 us in 4 pieces; 128 tokens 31 and 23 us. Where B and C do
         // not travel ahead in scalar registers a lone wavefront waits for them: 17 sequences (544 wavefronts)
-        // of 32 states 309 us uncut, 181 in 7 pieces; fp64 12 states 723 and 430.
+        // of 32 states 312 us uncut, 175 in 7 pieces; fp64 12 states 506 and 335.
         const bool early = q.lanes == 1 && N == q.npl && N * dtype_size(a->dtype) <= 64;
         if (w <= (early ? kUnits / 2 : kUnits * 5 / 8) && w > 0 && L >= 96)
             q.pieces = (int)std::min(4 * kUnits / w, L / 16);
