@@ -496,7 +496,8 @@ int cnh_fill_uniform_tile(double* out, int ndims, const int64_t* ext, const int6
 
 /* r = x + residual; y = r / sqrt(mean over the row of r^2 + eps) * weight. residual, residual_out and
  * weight (ones) are optional; residual_out receives r and may be the residual itself. The squares are
- * summed in the rows' own type: a sum beyond its range makes a row of zeros, as 1 / infinity does. */
+ * summed in the rows' own type: a sum beyond its range makes a row of zeros, as 1 / infinity does, and squares
+ * below it count as zeros. An eps below its smallest number counts as that. */
 typedef struct cnh_rms_norm_args {
     int32_t dtype;
     int64_t rows, cols;
@@ -544,8 +545,10 @@ int cnh_short_convolution(const cnh_short_convolution_args* a, cnh_stream s);
  * (device, 16-byte aligned, undefined contents before and after) then holds the bytes
  * cnh_state_scan_workspace asks for (it looks at the type and the sizes alone and needs no device).
  * Calls that may run at the same time need workspaces of their own, captured graphs among them. The
- * cut depends on the sizes alone; an output's last bits can differ between batch sizes. Tokens of a
- * sequence are less than 2 GiB apart in every operand (-3). */
+ * cut depends on the sizes alone; an output's last bits can differ between batch sizes. A and the steps may have
+ * either sign; states may grow, and leave the type's range only where their own value does. A rate of
+ * -infinity forgets at once and a step of 0 is no decay, whatever the rate; fp64 steps and rates are held to
+ * 1e22. Tokens of a sequence are less than 2 GiB apart in every operand (-3). */
 typedef struct cnh_state_scan_args {
     int32_t dtype, softplus;
     int64_t batch, length, channels, states;
@@ -583,7 +586,10 @@ int cnh_state_scan(const cnh_state_scan_args* a, cnh_stream s);
  * multiples of 2^-45 (of 2^-40 for 2^22 words), words more than 32 temperatures below the largest logit have none.
  * The scalars apply to every row; an array (device, one entry per row) takes the place of its scalar,
  * and an entry outside its range is held to it (a temperature that is not positive takes the largest
- * logit). `workspace` as for cnh_state_scan. */
+ * logit). `workspace` is used like cnh_state_scan's, but what cnh_sample_tokens_workspace asks for depends on the
+ * settings too: on top_k and temperature, and on whether top_ks and temperatures are there. The number it gives for
+ * top_k 0 and temperature 1 is the most that any settings need at that type and those sizes, for a caller
+ * who keeps one workspace for all requests. */
 typedef struct cnh_sample_tokens_args {
     int32_t dtype, top_k;
     int64_t rows, vocab;
