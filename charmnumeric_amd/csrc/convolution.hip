@@ -9,7 +9,7 @@
 // before the first is used; the taps - 1 rows before its first one are read a second time by the wavefront
 // before it, mostly from the caches (3 in 11 rows for 4 taps). The runs cut a long prompt too, so that it
 // fills the device. Short calls are bound by the launch and by fetching the code: hence few branches.
-// 4 x 2048 x 4096 in fp32, 4 taps, silu: 44 us, 6.0 TB/s of x and y. One token of 64 x 4096: 4.0 us.
+// 4 x 2048 x 4096 in fp32, 4 taps, silu: 45 us, 6.0 TB/s of x and y. One token of 64 x 4096: 4.1 us.
 #include "sequence.h"
 
 #include <algorithm>
@@ -161,8 +161,8 @@ int run(const cnh_short_convolution_args* a, hipStream_t st) {
         return !ptr || (aligned_to(ptr, 16) && (p.batch == 1 || outer % W == 0) && (p.length <= 1 || inner % W == 0));
     };
     // Up to 64 channels fit a wavefront one to a lane, and packs would leave most lanes idle: 61 x 1024 tokens of
-    // 64 channels take 9.3 us in fp32 and 14.6 in fp64, 12.4 and 18.4 in packs. 62 x 1024 of 96 take 14.0 and
-    // 22.7, 13.3 and 23.1 in packs, and wider rows are faster in packs.
+    // 64 channels take 9.4 us in fp32 and 15.3 in fp64, 14.1 and 19.4 in packs. 62 x 1024 of 96 take 14.3 and
+    // 24.4, 14.4 and 23.8 in packs, and wider rows are faster in packs.
     if (p.channels > 64 && p.channels % W == 0 && fits(p.x, p.x_batch_stride, p.x_stride) && fits(p.y, p.y_batch_stride, p.y_stride) &&
         fits(p.weight, 0, 0) && fits(p.bias, 0, 0) && fits(p.state_in, 0, 0) && fits(p.state_out, 0, 0))
         return launch_taps<T, W>(p, a->taps, a->activation != 0, st);

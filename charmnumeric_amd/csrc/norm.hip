@@ -12,7 +12,7 @@
 // A row gets one wavefront up to four packs a lane (1024 fp32 columns in 16-byte packs), four wavefronts up
 // to eight packs a lane, sixteen beyond: one wavefront for 2048 columns took 110 us where four take
 // 95.5 (16384 rows with a residual: 537 MB, 5.6 TB/s). 4 rows of 1024: 3.5 us, of which the launch and the
-// fetching of the code are most. 777 odd rows of 1537 fp64: 7.8 us, 19 MB at 2.4 TB/s.
+// fetching of the code are most. 777 odd rows of 1537 fp64: 8.2 us, 19 MB at 2.3 TB/s in accesses of one element.
 #include "sequence.h"
 
 #include <algorithm>

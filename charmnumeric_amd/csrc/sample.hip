@@ -21,11 +21,12 @@
 // Few rows whose every word has to be weighed are cut into slices: a pass for the slices' maxima, one that
 // adds their weights up bin by bin in the workspace, and the row's own workgroup goes on from there.
 //
-// A row is one workgroup's: what bounds it is the 62 GB/s that one CU reads, the 64-bit arithmetic of the
-// weighing, and some twenty short phases that each wait for their instructions. One row of 131072 fp32
-// words with a top-k of 50: 18.4 us (two passes of 4.2 us are memory). 256 rows of 50021, settings mixed:
-// 34.8 us, the time of a row that has to be weighed; 256 of 1000 words, sorted whole: 12.8 us. One row of
-// 131072 without a top-k, in 16 slices: 4 + 6 + 15.5 us.
+// A row is one workgroup's, on one CU: what bounds it is that CU's rate of reading (two sweeps of a greedy draw over
+// rows of 64 K to 256 K fp32 words: 150 GB/s, out of its L2; 80 to 105 GB/s over rows of 0.5 to 4 M words), the
+// 64-bit arithmetic of the weighing, and some twenty short phases that each wait for their instructions. One row of
+// 131072 fp32 words with a top-k of 50: 17.5 us, 7 of them its two sweeps. 256 rows of 50021, settings mixed:
+// 34.4 us, the time of a row that has to be weighed; 256 of 1000 words, sorted whole: 12.0 us. One row of 131072
+// without a top-k, in 16 slices: 4 + 6 + 20 us, with a top-p of 0.95 5 + 5 + 26.
 #include "sequence.h"
 
 #include <algorithm>

@@ -20,9 +20,11 @@
 // for prompts below 96 tokens.
 //
 // Prompts are bound by vector issue: a state of a token takes an exponential of 8.5 cycles and three to four
-// operations of 4.3 to 5. One prompt of 8192 tokens, 2048 channels and 16 fp32 states, in 128 pieces: 59 us for
-// what the pieces leave, 11 for their first states, 76 for the scan, vector issue busy 85 % of the time.
-// One token of 128 x 4096 channels is bound by the states: 13.4 us, 75 MB at 5.6 TB/s.
+// operations of 4.3 to 5. One prompt of 8192 tokens, 2048 channels and 16 fp32 states, in 128 pieces: 60 us for
+// what the pieces leave, 12 for their first states, 80 for the scan, vector issue busy 87 to 89 % of the time.
+// Padded prompts leave it idle more (65 to 72 %): pieces are cut over the padded length, and those behind a
+// sequence's end have nothing to do. One token of 128 x 4096 channels is bound by the states: 13.4 us, 75 MB at
+// 5.6 TB/s.
 #include "sequence.h"
 
 #include <algorithm>
@@ -504,8 +506,9 @@ __global__ __launch_bounds__(64) void scan_kernel(ScanParams<T> p) {
 // The state each piece starts from, in place of the one it leaves: 64 channels of one state per workgroup,
 // up to kSegments x GROUP pieces a round (as many segments as the pieces need). A lane loads its GROUP
 // pieces at once, folds them to one, takes what the segments before it leave from shared memory and walks
-// its pieces again in registers. 128 pieces of 2048 x 16 fp32 states: 11.9 us; with one lane per channel
-// that walks all pieces by itself and waits for memory once per GROUP of them 22.5 us.
+// its pieces again in registers. 128 pieces of 2048 x 16 fp32 states: 11.9 us (10.7 with decays that left the
+// type's range; 22.5 then with one lane per channel that walks all pieces by itself and waits for memory once per
+// GROUP of them).
 constexpr int kSegments = 8, kGroup = 8;
 template <typename T>
 __global__ __launch_bounds__(64 * kSegments) void carry_kernel(ScanParams<T> p) {
