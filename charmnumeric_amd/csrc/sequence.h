@@ -201,7 +201,7 @@ __device__ __forceinline__ double exp_of_minus(double x) {
 
 // x * sigmoid(x). In 32 bits e^-x is the hardware's 2^t for the rounded t = -x log2(e), with what the rounding left,
 // r = -x - t log(2), put in; without it the result is off by |x| half steps (18 on [-20, -10]). t is held to what 2^t can
-// be: r makes up for it where x is below -87, until the reciprocal is 0 (results of 2^-120 and less; it has no
+// be: r makes up for it where x is below -87, until the reciprocal is 0 (results of 2^-119 and less; it has no
 // denormals). The maximum is for 0 times infinity, at x = infinity.
 __device__ __forceinline__ float silu(float x) {
     const float t = __builtin_amdgcn_fmed3f(x * -1.44269504088896341f, -150.0f, 126.0f);

@@ -516,9 +516,10 @@ int cnh_rms_norm(const cnh_rms_norm_args* a, cnh_stream s);
 
 /* Causal convolution of every channel along its tokens with 1 to 8 taps:
  *   y[b, t, c] = act(bias[c] + sum over k < taps of weight[k, c] * x[b, t - (taps - 1) + k, c])
- * act: activation 0 none, 1 v * sigmoid(v). The rows in front of the first token come from
- * state_in (batch, taps - 1, channels; null: zeros); state_out receives the last taps - 1 rows of each
- * sequence, state included, and may be state_in itself. length 1 is one token per sequence. */
+ * act: activation 0 none, 1 v * sigmoid(v) (in fp32 0 where that is 2^-119 or less). The rows in front
+ * of the first token come from state_in (batch, taps - 1, channels; null: zeros); state_out receives the
+ * last taps - 1 rows of each sequence, state included, and may be state_in itself. length 1 is one token
+ * per sequence. */
 typedef struct cnh_short_convolution_args {
     int32_t dtype, activation, taps;
     int64_t batch, length, channels;
@@ -582,7 +583,8 @@ int cnh_state_scan(const cnh_state_scan_args* a, cnh_stream s);
  * those, in descending order, whose sum reaches top_p of theirs (one word at least); then min_p > 0 keeps
  * w >= min_p. out[row] is the first word, in descending order, at which the running sum of the kept
  * weights exceeds u[row] times their sum. A temperature of 0 takes the largest logit (ties: the lowest
- * index). -inf and NaN are never drawn; a row of nothing else gives -1. Weights are compared as
+ * index). -inf and NaN are never drawn; a row of nothing else gives -1. A difference of fp64 logits that is
+ * beyond the type's range is infinite, whatever the temperature. Weights are compared as
  * multiples of 2^-45 (of 2^-40 for 2^22 words), words more than 32 temperatures below the largest logit have none.
  * The scalars apply to every row; an array (device, one entry per row) takes the place of its scalar,
  * and an entry outside its range is held to it (a temperature that is not positive takes the largest
